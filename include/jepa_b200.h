@@ -146,6 +146,87 @@ int jepa_b200_attention_bench(int n_cand, int n_frames, int rows, int heads, int
 void jepa_b200_kprof_begin(void);
 int jepa_b200_kprof_end(char * out, size_t cap);
 
+// ---- A paged key / value cache held in 4 bits, for sessions of different lengths -------------------------------
+//
+// The entry points of this block work on DEVICE memory of the current device, on the caller's `stream` (a
+// cudaStream_t; null = the legacy default stream), allocate nothing and do not synchronise, so they can be captured
+// into a CUDA graph. They check their host arguments and that each pointer is memory of the current device; what lies
+// in device memory (lengths, slots, page ids) is bounds-checked by the kernels. No counterpart in the reference.
+//
+// A pool of n_pages pages of page_size token rows; slot s is row s % page_size of page s / page_size. Layout:
+//   q  uint8 [n_pages][2][kv_heads][page_size][head_dim / 2]   4-bit codes, low nibble first; plane 0 keys, 1 values
+//   d  f16   [n_pages][2][kv_heads][head_dim / 32][page_size]  one scale per 32 channels of a row
+// A code c stands for d (c - 8). Value rows keep their channels in order; a key row is a sequence of 8-channel words
+// of which word t NG + g holds channels 32 g + 8 t .. + 7 (NG = head_dim / 32, t = 0 .. 3).
+// 0.5625 bytes a value; both buffers must be 16-byte aligned (jepa_b200_kv4_bytes gives their sizes).
+typedef struct jepa_b200_kv4_cache {
+    void * q;
+    void * d;
+    int64_t n_pages;      // 1 .. 2^31 - 1
+    int32_t page_size;    // 16, 32, 64, 128 or 256
+    int32_t kv_heads;     // 1 .. 1024
+    int32_t head_dim;     // 32, 64, 96 or 128
+} jepa_b200_kv4_cache;
+
+int jepa_b200_kv4_bytes(const jepa_b200_kv4_cache * cache, size_t * q_bytes, size_t * d_bytes);
+
+// The bookkeeping of one step, built on the device: request r holds cached[r] tokens in the pages named by the first
+// ceil(cached[r] / page_size) entries of its row of `table` [n_req][width], and gets added[r] more (0 is allowed).
+// Fresh pages are taken from the start of free_pages [n_free], request by request, and written behind the held ones.
+//   lens [n_req]          cached + added
+//   q_start [n_req + 1]   exclusive sums of added: request r's new rows are q_start[r] .. q_start[r + 1] - 1
+//   slots [n_slots]       the slot of every new row, in that order; -1 behind the last (and for a negative page id)
+//   state [2]             {0, number of pages taken}, or {code, 0} of a refused step: 1 a negative length, 2 a request
+//                         outgrows its table row (or 2^31), 3 too few free pages, 4 more than n_slots new rows
+// A refused step (the smallest code of those that apply) leaves `table` as it was, sets lens = cached, q_start = 0 and
+// slots = -1, so that the calls behind it store and compute nothing. Table entries behind the taken pages stay as
+// they were. The arrays must not overlap. n_req, width, n_slots >= 1.
+int jepa_b200_kv_tables(const int32_t * cached, const int32_t * added, int n_req, int page_size, int32_t * table, int width,
+                        const int32_t * free_pages, int n_free, int32_t * lens, int32_t * q_start, int64_t * slots, int n_slots,
+                        int32_t * state, void * stream);
+
+// Quantises n_tokens rows of keys and values into their slots. k, v: ggml type 0 (f32), 1 (f16) or 30 (bf16), element
+// (token, head, channel) at token * tok + head * head_stride + channel (strides in elements). Per 32 channels: m = the
+// value of largest magnitude (the positive one of two), d = m / -8 rounded to bf16, then f16, and clamped to +-8160;
+// code = clamp(floor(x / d + 1/2) + 8, 0, 15), and 8 where d = 0. A group that holds an infinity or a NaN reads back as
+// NaN. Rows whose slot is negative or behind the pool are skipped. The slots of one call must differ: of two rows with
+// one slot, which one is kept is not defined (and may differ between groups).
+int jepa_b200_kv4_store(const jepa_b200_kv4_cache * cache, const void * k, const void * v, uint32_t type, int64_t k_tok, int64_t k_head,
+                        int64_t v_tok, int64_t v_head, const int64_t * slots, int64_t n_tokens, void * stream);
+
+// Reads rows back: k, v [n_tokens][kv_heads][head_dim], contiguous and 16-byte aligned, of the given type (f16 and f32
+// hold the cached values exactly; bf16 rounds them). A slot outside the pool reads as zeros; slots may repeat.
+int jepa_b200_kv4_load(const jepa_b200_kv4_cache * cache, const int64_t * slots, int64_t n_tokens, void * k, void * v, uint32_t type,
+                       void * stream);
+
+// Attention of every request's new rows over its cached rows (the new ones among them: store first).
+// Row i of the n = q_start[r + 1] - q_start[r] rows of request r stands at position p = lens[r] - n + i. It sees the
+// keys j < lens[r]; with frame > 0 only those with j < (p / frame + 1) * frame (block-causal over frames of that many
+// tokens; 1 = causal), and none when p < 0. A row that sees nothing gets zeros. Query heads are n_heads / kv_heads
+// consecutive ones for each cache head. Rows of out outside every request's range are left as they were. A page id
+// outside the pool leaves its keys out; lens is taken as at most width * page_size.
+typedef struct jepa_b200_kv4_attn {
+    const void * q;           // rows of `type`, element (row, head, channel) at row * q_tok + head * q_head + channel
+    void * out;               // the same type, with its own strides; must not overlap q
+    int64_t q_tok, q_head, o_tok, o_head;
+    const int32_t * q_start;  // [n_req + 1], ascending from 0
+    const int32_t * lens;     // [n_req]
+    const int32_t * table;    // [n_req][width]
+    int32_t n_req;            // 0 .. 65535
+    int32_t n_rows;           // rows of q and out
+    int32_t width;
+    int32_t n_heads;          // a multiple of kv_heads
+    uint32_t type;            // 1 (f16) or 30 (bf16)
+    int32_t frame;            // 0 = every cached key
+    float scale;              // of the scores, usually 1 / sqrt(head_dim)
+    int32_t max_len;          // bounds of lens and of rows per request that the launch is laid out for (0 = unknown):
+    int32_t max_new;          // larger ones are computed all the same, with less of the GPU
+    void * workspace;         // device, 16-byte aligned, jepa_b200_kv4_attention_workspace bytes; nothing is kept in
+    size_t workspace_bytes;   // it between calls, but calls that may run at once need one each
+} jepa_b200_kv4_attn;
+int64_t jepa_b200_kv4_attention_workspace(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args);
+int jepa_b200_kv4_attention(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, void * stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

@@ -1,0 +1,425 @@
+// Store and load of the 4-bit key / value cache, and the block tables and slot maps of a step (kv4.h).
+#include "kv4.h"
+#include "common.h"
+#include "launch.h"
+#include "kprof.h"
+
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+namespace jb {
+
+namespace {
+
+// ------------------------------------------------------------------------------------------
+// Store and load. A warp takes 8 tokens of one head, 4 lanes a token; lane t of a token holds channels
+// 32 g + 8 t .. + 7 of every group g. So the 4 lanes of a token agree on a group's scale with two shuffles, a
+// lane's key words lie side by side in the row, and the 8 tokens' scales of a group are 8 neighbours in memory
+// (when the tokens are neighbours in a page, as the rows of a sequence are).
+// ------------------------------------------------------------------------------------------
+
+template <class T> struct Vec8;
+template <> struct Vec8<__half> { uint4 a; };
+template <> struct Vec8<__nv_bfloat16> { uint4 a; };
+template <> struct Vec8<float> { uint4 a, b; };
+
+// 8 elements from p; vec: p is 16-byte aligned
+template <class T>
+__device__ __forceinline__ Vec8<T> load8(const T * p, bool vec) {
+    Vec8<T> v;
+    if (vec) {
+        v = *(const Vec8<T> *) p;
+    } else {
+        T e[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) e[i] = p[i];
+        memcpy(&v, e, sizeof(v));
+    }
+    return v;
+}
+
+template <class T>
+__device__ __forceinline__ void unpack8(const Vec8<T> & v, float (&x)[8]);
+template <> __device__ __forceinline__ void unpack8(const Vec8<float> & v, float (&x)[8]) { memcpy(x, &v, 32); }
+template <> __device__ __forceinline__ void unpack8(const Vec8<__half> & v, float (&x)[8]) {
+    const __half2 * h = (const __half2 *) &v;
+#pragma unroll
+    for (int i = 0; i < 4; i++) { const float2 f = __half22float2(h[i]); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
+}
+template <> __device__ __forceinline__ void unpack8(const Vec8<__nv_bfloat16> & v, float (&x)[8]) {
+    const __nv_bfloat162 * h = (const __nv_bfloat162 *) &v;
+#pragma unroll
+    for (int i = 0; i < 4; i++) { const float2 f = __bfloat1622float2(h[i]); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
+}
+
+// maximum and minimum that keep a NaN
+__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+
+// The scale of a group whose largest and smallest values are hi and lo: the value of largest magnitude (the positive
+// one of two) over -8, so that it takes code 0 and the 16 codes are used in full; rounded to bf16 (8 significant bits,
+// see kv4.h), then to f16, which the clamp keeps in range (8160 * 8 < 65504). A group with an infinity or a NaN gets NaN.
+__device__ __forceinline__ __half group_scale(float hi, float lo) {
+    const float m = hi >= -lo ? hi : lo;
+    const float r = __bfloat162float(__float2bfloat16_rn(m * -0.125f));
+    const float d = fminf(fmaxf(r, -8160.0f), 8160.0f);
+    const bool finite = hi - hi == 0.0f && lo - lo == 0.0f;   // false for infinities and NaN
+    return finite ? __float2half_rn(d) : __ushort_as_half((unsigned short) 0x7fff);
+}
+
+// code = clamp(floor(x / d + 1/2) + 8, 0, 15).
+// For f16 and bf16 x the quotient of an 11-bit by an 8-bit significand is a half-integer or at least 2^-13 away
+// from one (for |quotient| between 1/2 and 8.1), and x * inv is within 2^-19 of it: adding 2^-15 decides every case as the
+// exact quotient would. For f32 x the estimate is corrected by the sign of x - (c -+ 1/2) d, one fused rounding each.
+template <class T>
+__device__ __forceinline__ uint32_t code_of(float x, float d, float inv) {
+    float t = __fmaf_rn(x, inv, 8.5f + 0x1p-15f);
+    t = fminf(fmaxf(t, 0.0f), 15.5f);
+    uint32_t c = __float_as_uint(__fadd_rd(t, 8388608.0f)) & 15u;   // floor, in the low bits of 2^23 + t
+    if (sizeof(T) == 4) {
+        const float s = d < 0.0f ? -1.0f : 1.0f;
+        const float k = (float) c - 8.0f;
+        const float below = __fmaf_rn(-(k - 0.5f), d, x) * s, above = __fmaf_rn(-(k + 0.5f), d, x) * s;
+        if (below < 0.0f && c > 0) c--;
+        else if (above >= 0.0f && c < 15) c++;
+    }
+    return c;
+}
+
+template <class T, int NG>
+__device__ __forceinline__ void quantise_row(const Vec8<T> (&in)[NG], uint32_t (&word)[NG], __half (&scale)[NG]) {
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        float x[8];
+        unpack8<T>(in[g], x);
+        float hi = x[0], lo = x[0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) { hi = max_nan(hi, x[i]); lo = min_nan(lo, x[i]); }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        }
+        scale[g] = group_scale(hi, lo);
+        const float d = __half2float(scale[g]);
+        const bool zero = d == 0.0f || d != d;
+        const float inv = zero ? 0.0f : __fdiv_rn(1.0f, d);
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) w |= code_of<T>(x[i], d, inv) << (4 * i);
+        word[g] = zero ? 0x88888888u : w;
+    }
+}
+
+template <class T, int NG>
+__global__ void __launch_bounds__(128) k_kv4_store(const Kv4Pool p, const Kv4Rows r, const int64_t * __restrict__ slots, long long n,
+                                                   bool vec) {
+    constexpr int HD = 32 * NG;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int lane = threadIdx.x & 31, t = lane & 3;
+    const long long task = (long long) blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const int h = (int) (task % p.heads);
+    const long long tok = (task / p.heads) * 8 + (lane >> 2);
+    if (task / p.heads * 8 >= n) return;                       // the whole warp
+    const long long slot = tok < n ? slots[tok] : -1;
+    const bool live = slot >= 0 && slot < p.n_slots;
+    const long long row = live ? tok : task / p.heads * 8;     // a row that exists, for the shuffles' sake
+    const T * k = (const T *) r.k + row * r.k_tok + h * r.k_head + 8 * t;
+    const T * v = (const T *) r.v + row * r.v_tok + h * r.v_head + 8 * t;
+    Vec8<T> kin[NG], vin[NG];
+#pragma unroll
+    for (int g = 0; g < NG; g++) kin[g] = load8<T>(k + 32 * g, vec);
+#pragma unroll
+    for (int g = 0; g < NG; g++) vin[g] = load8<T>(v + 32 * g, vec);
+    uint32_t kw[NG], vw[NG];
+    __half ks[NG], vs[NG];
+    quantise_row<T, NG>(kin, kw, ks);
+    quantise_row<T, NG>(vin, vw, vs);
+    if (!live) return;
+    const long long page = slot >> p.page_shift;
+    const int at = (int) (slot & ((1 << p.page_shift) - 1)), P = 1 << p.page_shift;
+    uint32_t * kq = (uint32_t *) (p.q + kv4_q_at(p, page, 0, h, at)) + t * NG;
+    if (NG == 4) *(uint4 *) kq = make_uint4(kw[0], kw[1 % NG], kw[2 % NG], kw[3 % NG]);
+    else if (NG == 2) *(uint2 *) kq = make_uint2(kw[0], kw[1 % NG]);
+    else {
+#pragma unroll
+        for (int g = 0; g < NG; g++) kq[g] = kw[g];
+    }
+    uint32_t * vq = (uint32_t *) (p.q + kv4_q_at(p, page, 1, h, at));
+#pragma unroll
+    for (int g = 0; g < NG; g++) vq[4 * g + t] = vw[g];
+    __half * kd = p.d + kv4_d_at(p, page, 0, h, at);
+    __half * vd = p.d + kv4_d_at(p, page, 1, h, at);
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        if (t == g) { kd[(size_t) g * P] = ks[g]; vd[(size_t) g * P] = vs[g]; }
+    }
+    (void) HD;
+}
+
+template <class T> __device__ __forceinline__ T to_type(float x);
+template <> __device__ __forceinline__ float to_type(float x) { return x; }
+template <> __device__ __forceinline__ __half to_type(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 to_type(float x) { return __float2bfloat16_rn(x); }
+
+// 8 values d (c - 8) of one word, rounded once to T (f16 and f32 hold them exactly)
+template <class T>
+__device__ __forceinline__ void write8(T * p, uint32_t w, float d, bool live) {
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) e[i] = to_type<T>(live ? (float) ((int) ((w >> (4 * i)) & 15u) - 8) * d : 0.0f);
+    Vec8<T> v;
+    memcpy(&v, e, sizeof(v));
+    *(Vec8<T> *) p = v;
+}
+
+template <class T, int NG>
+__global__ void __launch_bounds__(128) k_kv4_load(const Kv4Pool p, T * __restrict__ ko, T * __restrict__ vo,
+                                                  const int64_t * __restrict__ slots, long long n) {
+    constexpr int HD = 32 * NG;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int lane = threadIdx.x & 31, t = lane & 3;
+    const long long task = (long long) blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const int h = (int) (task % p.heads);
+    const long long tok = (task / p.heads) * 8 + (lane >> 2);
+    if (tok >= n) return;
+    const long long slot = slots[tok];
+    const bool live = slot >= 0 && slot < p.n_slots;
+    const long long page = live ? slot >> p.page_shift : 0;
+    const int at = live ? (int) (slot & ((1 << p.page_shift) - 1)) : 0, P = 1 << p.page_shift;
+    const uint32_t * kq = (const uint32_t *) (p.q + kv4_q_at(p, page, 0, h, at)) + t * NG;
+    const uint32_t * vq = (const uint32_t *) (p.q + kv4_q_at(p, page, 1, h, at)) + t;
+    const __half * kd = p.d + kv4_d_at(p, page, 0, h, at);
+    const __half * vd = p.d + kv4_d_at(p, page, 1, h, at);
+    uint32_t kw[NG], vw[NG];
+    float ks[NG], vs[NG];
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        kw[g] = kq[g];
+        vw[g] = vq[4 * g];
+        ks[g] = __half2float(kd[(size_t) g * P]);
+        vs[g] = __half2float(vd[(size_t) g * P]);
+    }
+    const size_t o = ((size_t) tok * p.heads + h) * HD + 8 * t;
+#pragma unroll
+    for (int g = 0; g < NG; g++) write8<T>(ko + o + 32 * g, kw[g], ks[g], live);
+#pragma unroll
+    for (int g = 0; g < NG; g++) write8<T>(vo + o + 32 * g, vw[g], vs[g], live);
+}
+
+template <class T, int NG>
+int store_launch(const Kv4Pool & p, const Kv4Rows & r, const int64_t * slots, long long n, dim3 grid, cudaStream_t st) {
+    const long long strides = r.k_tok | r.k_head | r.v_tok | r.v_head;
+    const bool vec = (((uintptr_t) r.k | (uintptr_t) r.v) & 15) == 0 && (strides * (long long) sizeof(T)) % 16 == 0;
+    JB_CUDA(launch_pdl(k_kv4_store<T, NG>, grid, dim3(128), 0, st, p, r, slots, n, vec));
+    return 0;
+}
+template <class T, int NG>
+int load_launch(const Kv4Pool & p, const Kv4Rows & r, const int64_t * slots, long long n, dim3 grid, cudaStream_t st) {
+    JB_CUDA(launch_pdl(k_kv4_load<T, NG>, grid, dim3(128), 0, st, p, (T *) r.k, (T *) r.v, slots, n));
+    return 0;
+}
+
+template <class T>
+int store_dim(const Kv4Pool & p, const Kv4Rows & r, const int64_t * slots, long long n, dim3 grid, cudaStream_t st) {
+    switch (p.hd / 32) {
+        case 1: return store_launch<T, 1>(p, r, slots, n, grid, st);
+        case 2: return store_launch<T, 2>(p, r, slots, n, grid, st);
+        case 3: return store_launch<T, 3>(p, r, slots, n, grid, st);
+        default: return store_launch<T, 4>(p, r, slots, n, grid, st);
+    }
+}
+template <class T>
+int load_dim(const Kv4Pool & p, const Kv4Rows & r, const int64_t * slots, long long n, dim3 grid, cudaStream_t st) {
+    switch (p.hd / 32) {
+        case 1: return load_launch<T, 1>(p, r, slots, n, grid, st);
+        case 2: return load_launch<T, 2>(p, r, slots, n, grid, st);
+        case 3: return load_launch<T, 3>(p, r, slots, n, grid, st);
+        default: return load_launch<T, 4>(p, r, slots, n, grid, st);
+    }
+}
+
+double row_bytes(const Kv4Pool & p, int type) {
+    return 2.0 * p.heads * p.hd * ((type == KV4_F32 ? 4 : 2) + 0.5625) + 8;
+}
+
+}  // namespace
+
+int kv4_store(const Kv4Pool & p, const Kv4Rows & r, int type, const int64_t * slots, long long n, cudaStream_t st) {
+    if (n < 1) return 0;
+    const long long blocks = ((n + 7) / 8 * p.heads + 3) / 4;
+    if (blocks > 0x7fffffffLL) { log("jepa: jepa_b200_kv4_store: %lld tokens are too many for one call\n", n); return -1; }
+    KTimer kt("kv4_store", st, 0, row_bytes(p, type) * n);
+    const dim3 grid((unsigned) blocks);
+    switch (type) {
+        case KV4_F32: return store_dim<float>(p, r, slots, n, grid, st);
+        case KV4_F16: return store_dim<__half>(p, r, slots, n, grid, st);
+        default: return store_dim<__nv_bfloat16>(p, r, slots, n, grid, st);
+    }
+}
+
+int kv4_load(const Kv4Pool & p, const Kv4Rows & r, int type, const int64_t * slots, long long n, cudaStream_t st) {
+    if (n < 1) return 0;
+    const long long blocks = ((n + 7) / 8 * p.heads + 3) / 4;
+    if (blocks > 0x7fffffffLL) { log("jepa: jepa_b200_kv4_load: %lld tokens are too many for one call\n", n); return -1; }
+    KTimer kt("kv4_load", st, 0, row_bytes(p, type) * n);
+    const dim3 grid((unsigned) blocks);
+    switch (type) {
+        case KV4_F32: return load_dim<float>(p, r, slots, n, grid, st);
+        case KV4_F16: return load_dim<__half>(p, r, slots, n, grid, st);
+        default: return load_dim<__nv_bfloat16>(p, r, slots, n, grid, st);
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// Block tables and slot maps of a step
+// ------------------------------------------------------------------------------------------
+
+namespace {
+
+constexpr int TAB_THREADS = 512;
+
+struct TokPg { long long tok, pg; };
+
+// inclusive scan over the block of one pair per thread; `total` receives the block's sums
+__device__ __forceinline__ TokPg block_scan(TokPg x, TokPg & total, TokPg * warp_sum) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long a = __shfl_up_sync(0xffffffffu, x.tok, o), b = __shfl_up_sync(0xffffffffu, x.pg, o);
+        if (lane >= o) { x.tok += a; x.pg += b; }
+    }
+    __syncthreads();                     // the array's last readers are done
+    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();
+    TokPg before = {0, 0};
+    total = {0, 0};
+    for (int w = 0; w < nw; w++) {
+        const TokPg s = warp_sum[w];
+        if (w < warp) { before.tok += s.tok; before.pg += s.pg; }
+        total.tok += s.tok;
+        total.pg += s.pg;
+    }
+    x.tok += before.tok;
+    x.pg += before.pg;
+    return x;
+}
+
+struct Request { int cached, added, held, need, bad; };
+
+__device__ __forceinline__ Request request_of(const KvTablesArgs & a, int r) {
+    Request q = {0, 0, 0, 0, 0};
+    if (r >= a.n_req) return q;
+    q.cached = a.cached[r];
+    q.added = a.added[r];
+    const int P1 = (1 << a.page_shift) - 1;
+    const long long len = (long long) q.cached + q.added;
+    if (q.cached < 0 || q.added < 0) q.bad = 1;
+    else if (len > (long long) a.width << a.page_shift || len > 0x7fffffffLL - P1) q.bad = 2;
+    if (q.bad) { q.added = 0; return q; }
+    q.held = (q.cached + P1) >> a.page_shift;
+    q.need = (int) ((len + P1) >> a.page_shift) - q.held;
+    return q;
+}
+
+// last index of v[0 .. n) (ascending, v[0] <= x) with v[i] <= x
+__device__ __forceinline__ int last_le(const int * v, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (v[mid] <= x) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// Every CTA walks all requests, TAB_THREADS a time, with a scan of their new tokens and new pages (two integers a
+// request: it stays in L2), and writes its own share of the flat outputs: slots and fresh table entries, each found by
+// bisection among the walked requests' first tokens / pages. One launch, no communication between CTAs, balanced however
+// unequal the requests are. A refused step (state[0] != 0) is known to every CTA before anything is written.
+__global__ void __launch_bounds__(TAB_THREADS) k_kv_tables(const KvTablesArgs a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ TokPg warp_sum[TAB_THREADS / 32];
+    __shared__ int first_tok[TAB_THREADS], first_pg[TAB_THREADS], s_cached[TAB_THREADS], s_held[TAB_THREADS];
+    __shared__ int s_bad;
+    const int tid = threadIdx.x, nt = blockDim.x;
+    const int n_chunks = (a.n_req + nt - 1) / nt;
+    if (tid == 0) s_bad = 0x7fffffff;
+    __syncthreads();
+    // totals and refusals (one chunk: the scan below gives them)
+    TokPg all = {0, 0};
+    Request q = request_of(a, tid);
+    {
+        TokPg mine = {q.added, q.need};
+        int bad = q.bad ? q.bad : 0x7fffffff;
+        for (int r = tid + nt; r < a.n_req; r += nt) {
+            const Request o = request_of(a, r);
+            mine.tok += o.added;
+            mine.pg += o.need;
+            if (o.bad) bad = min(bad, o.bad);
+        }
+        if (bad != 0x7fffffff) atomicMin(&s_bad, bad);
+        block_scan(mine, all, warp_sum);
+    }
+    __syncthreads();
+    int status = s_bad == 0x7fffffff ? 0 : s_bad;
+    if (!status && all.pg > a.n_free) status = 3;
+    if (!status && all.tok > a.n_slots) status = 4;
+    const int n_tok = status ? 0 : (int) all.tok, n_pg = status ? 0 : (int) all.pg;
+    if (blockIdx.x == 0 && tid == 0) {
+        a.state[0] = status;
+        a.state[1] = n_pg;
+        a.q_start[a.n_req] = n_tok;
+    }
+    const int s0 = (int) ((long long) a.n_slots * blockIdx.x / gridDim.x), s1 = (int) ((long long) a.n_slots * (blockIdx.x + 1) / gridDim.x);
+    const int p0 = (int) ((long long) n_pg * blockIdx.x / gridDim.x), p1 = (int) ((long long) n_pg * (blockIdx.x + 1) / gridDim.x);
+    for (int i = max(s0, n_tok) + tid; i < s1; i += nt) a.slots[i] = -1;
+    int tok0 = 0, pg0 = 0;                // first token and page of the chunk
+    for (int c = 0; c < n_chunks; c++) {
+        const int r0 = c * nt, r = r0 + tid, n = min(nt, a.n_req - r0);
+        if (c) q = request_of(a, r);
+        if (status) {
+            if (c % gridDim.x == blockIdx.x && r < a.n_req) { a.lens[r] = a.cached[r]; a.q_start[r] = 0; }
+            continue;
+        }
+        TokPg sum;
+        const TokPg inc = block_scan({q.added, q.need}, sum, warp_sum);
+        first_tok[tid] = tok0 + (int) inc.tok - q.added;
+        first_pg[tid] = pg0 + (int) inc.pg - q.need;
+        s_cached[tid] = q.cached;
+        s_held[tid] = q.held;
+        if (c % gridDim.x == blockIdx.x && r < a.n_req) { a.lens[r] = q.cached + q.added; a.q_start[r] = first_tok[tid]; }
+        __syncthreads();
+        const int tok1 = tok0 + (int) sum.tok, pg1 = pg0 + (int) sum.pg;
+        for (int i = max(p0, pg0) + tid; i < min(p1, pg1); i += nt) {
+            const int k = last_le(first_pg, n, i);
+            a.table[(size_t) (r0 + k) * a.width + s_held[k] + (i - first_pg[k])] = a.free_pages[i];
+        }
+        for (int i = max(s0, tok0) + tid; i < min(s1, tok1); i += nt) {
+            const int k = last_le(first_tok, n, i);
+            const int pos = s_cached[k] + (i - first_tok[k]), idx = pos >> a.page_shift;
+            // a page held before this step comes from the table, a fresh one from the free list
+            const int page = idx < s_held[k] ? a.table[(size_t) (r0 + k) * a.width + idx] : a.free_pages[first_pg[k] + idx - s_held[k]];
+            a.slots[i] = page < 0 ? -1 : ((long long) page << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+        }
+        tok0 = tok1;
+        pg0 = pg1;
+        __syncthreads();
+    }
+}
+
+}  // namespace
+
+int kv_tables(const KvTablesArgs & a, cudaStream_t st) {
+    KTimer kt("kv_tables", st, 0, 16.0 * a.n_req + 8.0 * a.n_slots);
+    // 4 slots a thread and more before another CTA joins; one CTA an SM at most (each walks every request)
+    const int threads = a.n_req <= 128 && a.n_slots <= 512 ? 128 : TAB_THREADS;
+    const int blocks = std::max(1, std::min(148, (a.n_slots + 4 * threads - 1) / (4 * threads)));
+    JB_CUDA(launch_pdl(k_kv_tables, dim3((unsigned) blocks), dim3((unsigned) threads), 0, st, a));
+    return 0;
+}
+
+}  // namespace jb

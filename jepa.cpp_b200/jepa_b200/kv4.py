@@ -1,0 +1,217 @@
+"""The paged 4-bit key / value cache on torch CUDA tensors: block tables and slot maps of a step, store, load, and the
+attention that reads the cache (include/jepa_b200.h, the kv4 block). Every call runs on the current stream of the
+tensors' device, without a synchronisation, and can be captured into a CUDA graph.
+
+    cache = KV4Cache(n_pages, page_size, kv_heads, head_dim)
+    t = build_tables(cached, added, table, free_pages, page_size, n_slots)   # new pages, slots, row ranges
+    cache.store(k, v, t.slots)                                              # this step's rows
+    out = cache.attention(q, t.q_start, t.lens, table, frame=258, max_new=258)
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from . import lib as jlib
+
+_TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+
+
+class _Cache(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("d", C.c_void_p), ("n_pages", C.c_int64), ("page_size", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class _Attn(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_tok", C.c_int64), ("q_head", C.c_int64), ("o_tok", C.c_int64),
+                ("o_head", C.c_int64), ("q_start", C.c_void_p), ("lens", C.c_void_p), ("table", C.c_void_p),
+                ("n_req", C.c_int32), ("n_rows", C.c_int32), ("width", C.c_int32), ("n_heads", C.c_int32),
+                ("type", C.c_uint32), ("frame", C.c_int32), ("scale", C.c_float), ("max_len", C.c_int32),
+                ("max_new", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+_lib: Optional[C.CDLL] = None
+
+
+def _load() -> C.CDLL:
+    global _lib
+    if _lib is None:
+        L = jlib.load()
+        vp, i32, i64, cp = C.c_void_p, C.c_int, C.c_int64, C.POINTER(_Cache)
+        sig = {
+            "jepa_b200_kv4_bytes": (i32, [cp, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]),
+            "jepa_b200_kv_tables": (i32, [vp, vp, i32, i32, vp, i32, vp, i32, vp, vp, vp, i32, vp, vp]),
+            "jepa_b200_kv4_store": (i32, [cp, vp, vp, C.c_uint32, i64, i64, i64, i64, vp, i64, vp]),
+            "jepa_b200_kv4_load": (i32, [cp, vp, i64, vp, vp, C.c_uint32, vp]),
+            "jepa_b200_kv4_attention_workspace": (i64, [cp, C.POINTER(_Attn)]),
+            "jepa_b200_kv4_attention": (i32, [cp, C.POINTER(_Attn), vp]),
+        }
+        for name, (res, args) in sig.items():
+            f = getattr(L, name)
+            f.restype, f.argtypes = res, args
+        _lib = L
+    return _lib
+
+
+def _call(name: str, dev: torch.device, *args) -> None:
+    """One call on the device's current stream (the C entry works on the current device)."""
+    L = _load()
+    fn = getattr(L, name)
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc != 0:
+        _raise(L, name)
+
+
+def _raise(L: C.CDLL, name: str) -> None:
+    text = (L.jepa_error_text() or b"").decode(errors="replace").strip().splitlines()
+    L.jepa_error_reset()
+    raise RuntimeError(text[-1] if text else f"{name} failed")
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _index(t: torch.Tensor, name: str, dtype: torch.dtype, dev: Optional[torch.device], dim: int = 1) -> None:
+    _need(isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == dim and t.is_contiguous(),
+          f"{name} must be a contiguous {dim}-D tensor of {dtype}")
+    _need(t.is_cuda and (dev is None or t.device == dev), f"{name} must be on the CUDA device of the others")
+
+
+class Tables(NamedTuple):
+    """What build_tables gives: the arrays that store and attention take, and state = [refusal code or 0, pages taken]."""
+    lens: torch.Tensor
+    q_start: torch.Tensor
+    slots: torch.Tensor
+    state: torch.Tensor
+
+
+def build_tables(cached: torch.Tensor, added: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor, page_size: int,
+                 n_slots: int) -> Tables:
+    """The bookkeeping of one step from the requests' lengths (int32, on the GPU): fresh pages from the start of
+    free_pages go into `table` [n_req, width] (changed in place), every new row gets its slot. n_slots is the size of
+    the slot map, at least the number of new rows; the rest is -1. A refused step (state[0] != 0) changes nothing and
+    gives empty row ranges: see jepa_b200_kv_tables."""
+    _index(cached, "cached", torch.int32, None)
+    dev, n = cached.device, cached.shape[0]
+    _index(added, "added", torch.int32, dev)
+    _index(table, "table", torch.int32, dev, 2)
+    _index(free_pages, "free_pages", torch.int32, dev)
+    _need(added.shape[0] == n and table.shape[0] == n, "cached, added and table must have one entry a request")
+    _need(n >= 1 and table.shape[1] >= 1, "there must be a request and a table column")
+    _need(1 <= n_slots < 2 ** 31, f"n_slots {n_slots} is not 1 .. 2^31 - 1")
+    # lens, q_start and state share one allocation, each at a multiple of 4 bytes
+    ints = torch.empty(2 * n + 3, dtype=torch.int32, device=dev)
+    lens, q_start, state = ints[:n], ints[n:2 * n + 1], ints[2 * n + 1:]
+    slots = torch.empty(n_slots, dtype=torch.int64, device=dev)
+    base = ints.data_ptr()
+    _call("jepa_b200_kv_tables", dev, cached.data_ptr(), added.data_ptr(), n, page_size, table.data_ptr(), table.shape[1],
+          free_pages.data_ptr(), free_pages.shape[0], base, base + 4 * n, slots.data_ptr(), n_slots, base + 4 * (2 * n + 1))
+    return Tables(lens, q_start, slots, state)
+
+
+class KV4Cache:
+    """A pool of pages of token rows whose keys and values are held in 4 bits (layout: include/jepa_b200.h)."""
+
+    def __init__(self, n_pages: int, page_size: int, kv_heads: int, head_dim: int, device="cuda"):
+        c = _Cache(None, None, n_pages, page_size, kv_heads, head_dim)
+        L, qb, db = _load(), C.c_size_t(), C.c_size_t()
+        if L.jepa_b200_kv4_bytes(C.byref(c), C.byref(qb), C.byref(db)) != 0:
+            _raise(L, "jepa_b200_kv4_bytes")
+        self._bind(torch.zeros((n_pages, 2, kv_heads, page_size, head_dim // 2), dtype=torch.uint8, device=device),
+                   torch.zeros((n_pages, 2, kv_heads, head_dim // 32, page_size), dtype=torch.float16, device=device))
+
+    @classmethod
+    def wrap(cls, q: torch.Tensor, d: torch.Tensor) -> "KV4Cache":
+        """A cache over buffers that exist: q uint8 [pages, 2, heads, page, dim / 2], d f16 [pages, 2, heads, dim / 32, page]."""
+        self = cls.__new__(cls)
+        self._bind(q, d)
+        return self
+
+    def _bind(self, q: torch.Tensor, d: torch.Tensor) -> None:
+        _index(q, "q", torch.uint8, None, 5)
+        _index(d, "d", torch.float16, q.device, 5)
+        n, two, heads, page, half = q.shape
+        _need(two == 2 and d.shape == (n, 2, heads, half // 16, page) and half % 16 == 0, "q and d do not belong to one layout")
+        self.q, self.d = q, d
+        self.n_pages, self.page_size, self.kv_heads, self.head_dim = n, page, heads, 2 * half
+        self._c = _Cache(q.data_ptr(), d.data_ptr(), n, page, heads, 2 * half)
+        L, qb, db = _load(), C.c_size_t(), C.c_size_t()
+        if L.jepa_b200_kv4_bytes(C.byref(self._c), C.byref(qb), C.byref(db)) != 0:
+            _raise(L, "jepa_b200_kv4_bytes")
+        _need(qb.value == q.numel() and db.value == 2 * d.numel(), "q and d do not belong to one layout")
+        self._ref = C.byref(self._c)
+        self._dev = q.device
+
+    def _rows(self, t: torch.Tensor, name: str, heads: int) -> None:
+        _need(isinstance(t, torch.Tensor) and t.dim() == 3 and t.shape[1] == heads and t.shape[2] == self.head_dim,
+              f"{name} must be [rows, {heads}, {self.head_dim}]")
+        _need(t.device == self._dev, f"{name} must be on {self._dev}")
+        _need(t.stride(2) == 1, f"{name}'s channels must be contiguous")
+
+    def store(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        """Quantise rows k, v [n, kv_heads, head_dim] (f32, f16 or bf16, any strides of rows and heads) into slots [n]
+        (int64; negative ones are skipped, the others must differ)."""
+        self._rows(k, "k", self.kv_heads)
+        self._rows(v, "v", self.kv_heads)
+        _index(slots, "slots", torch.int64, self._dev)
+        _need(k.dtype in _TYPE and v.dtype is k.dtype, "k and v must be both f32, f16 or bf16")
+        n = slots.shape[0]
+        _need(k.shape[0] == n and v.shape[0] == n, "k, v and slots must have one row a token")
+        _call("jepa_b200_kv4_store", self._dev, self._ref, k.data_ptr(), v.data_ptr(), _TYPE[k.dtype], k.stride(0), k.stride(1),
+              v.stride(0), v.stride(1), slots.data_ptr(), n)
+
+    def load(self, slots: torch.Tensor, dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The values cached in slots [n] (int64): k, v [n, kv_heads, head_dim]; zeros for a slot outside the pool."""
+        _index(slots, "slots", torch.int64, self._dev)
+        _need(dtype in _TYPE, f"{dtype} is not f32, f16 or bf16")
+        shape = (slots.shape[0], self.kv_heads, self.head_dim)
+        k = torch.empty(shape, dtype=dtype, device=self._dev)
+        v = torch.empty(shape, dtype=dtype, device=self._dev)
+        _call("jepa_b200_kv4_load", self._dev, self._ref, slots.data_ptr(), shape[0], k.data_ptr(), v.data_ptr(), _TYPE[dtype])
+        return k, v
+
+    def attention(self, q: torch.Tensor, q_start: torch.Tensor, lens: torch.Tensor, table: torch.Tensor,
+                  scale: Optional[float] = None, frame: int = 0, max_len: int = 0, max_new: int = 0,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of the rows q [rows, heads, head_dim] (f16 or bf16) over the cached rows of their requests:
+        request r owns rows q_start[r] .. q_start[r + 1] - 1 and the first lens[r] positions of table[r]. frame: 0 =
+        every cached key, 1 = causal, F = block-causal over frames of F tokens. max_len / max_new: bounds of lens and of
+        a request's rows, which the launch is laid out for (they change no result). out (zeros by default) keeps the
+        rows of no request."""
+        _need(q.dim() == 3, "q must be [rows, heads, head_dim]")
+        heads = q.shape[1]
+        self._rows(q, "q", heads)
+        _need(q.dtype is torch.float16 or q.dtype is torch.bfloat16, "q must be f16 or bf16")
+        _index(lens, "lens", torch.int32, self._dev)
+        _index(q_start, "q_start", torch.int32, self._dev)
+        _index(table, "table", torch.int32, self._dev, 2)
+        n = lens.shape[0]
+        _need(q_start.shape[0] == n + 1 and table.shape[0] == n, "lens, q_start and table must agree on the requests")
+        if out is None:
+            out = torch.zeros(q.shape, dtype=q.dtype, device=self._dev)
+        else:
+            self._rows(out, "out", heads)
+            _need(out.dtype is q.dtype and out.shape[0] == q.shape[0], "out must be of q's type and shape")
+        a = _Attn(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), q_start.data_ptr(),
+                  lens.data_ptr(), table.data_ptr(), n, q.shape[0], table.shape[1], heads, _TYPE[q.dtype], frame,
+                  1.0 / math.sqrt(self.head_dim) if scale is None else scale, max_len, max_new, None, 0)
+        ref = C.byref(a)
+        L = _load()
+        need = L.jepa_b200_kv4_attention_workspace(self._ref, ref)
+        if need < 0:
+            _raise(L, "jepa_b200_kv4_attention")
+        if need:
+            # from the caching allocator, on the stream of the call: two calls, or two graphs, never share it
+            ws = torch.empty(need, dtype=torch.uint8, device=self._dev)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        _call("jepa_b200_kv4_attention", self._dev, self._ref, ref)
+        return out
