@@ -3,6 +3,23 @@
 //   row i of request r (of n = q_start[r + 1] - q_start[r]) stands at position p = lens[r] - n + i and sees the keys
 //   j < lens[r], and with frame > 0 only j < (p / frame + 1) frame (none for p < 0):
 //   out = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q . k_j - max);  0 for a row that sees nothing.
+//
+// k_kv4_rows, for few rows: one pass over the cache, bound by its 0.5625 bytes a value. The query rows that share a
+// cache head (new tokens x the heads of its group) are columns of the products, 8 or 16 of them:
+//   S^T [16 keys x 8 rows]  = K [16 x hd] Q^T          mma m16n8k16, one accumulator per 32-channel group: the codes go
+//                                                 in as the integers -8 .. 7 (exact in f16), the group's scale
+//                                                 multiplies the f32 sum
+//   O^T [hd x 8 rows]      += V^T [hd x 16 keys] P^T   the operand is d (c - 8), exact in f16; P = 2^(s - m + 10) in
+//                                                 f16: the 2^10 keeps weights down to 2^-24 of the largest
+//                                                 normal, the 11 bits cost half an ulp of f16 a weight at most
+// Both products take the cache as the A operand, in the order in which it lies in memory: key rows for S^T (a lane's 8
+// channels of each group are one 4-byte word), and for O^T a pair of key rows' words merged nibble by nibble; P^T comes
+// from S^T by an 8 x 8 transpose inside the warp (movmatrix). Queries are scaled by a power of two per row into f16's
+// range (bf16 has 8 more exponent bits than it needs here), which the scores' factor undoes.
+// Each warp runs by itself over every fourth step of 32 keys of the CTA's range, fed by its own three-stage cp.async ring
+// (the four states are merged at the end); the maximum is raised, and the sums rescaled, only when a score passes it
+// by 2^4, so most steps do no reduction across lanes. A long context is split over CTAs, whose partial sums
+// k_kv4_merge joins.
 #include "kv4.h"
 #include "common.h"
 #include "launch.h"
@@ -10,95 +27,577 @@
 
 #include <cuda_bf16.h>
 
+#include <algorithm>
+#include <type_traits>
+
 namespace jb {
 
 namespace {
 
-__device__ __forceinline__ float from_type(__half x) { return __half2float(x); }
-__device__ __forceinline__ float from_type(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <class T> __device__ __forceinline__ T to_type(float x);
 template <> __device__ __forceinline__ __half to_type(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 to_type(float x) { return __float2bfloat16_rn(x); }
+__device__ __forceinline__ float from_type(__half x) { return __half2float(x); }
+__device__ __forceinline__ float from_type(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// keys row p (its position) sees
-__device__ __forceinline__ int visible(int p, int len, int frame) {
-    if (frame == 0) return len;
-    if (p < 0) return 0;
-    const long long lim = ((long long) p / frame + 1) * frame;
-    return lim < len ? (int) lim : len;
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-// one warp per (row, head), lane c holding channels c, c + 32, ..
-template <class T, int NG>
-__global__ void __launch_bounds__(128) k_kv4_attention(const Kv4Pool pool, const Kv4Attn a) {
+// how a request's keys are divided: n_split ranges of `chunk` keys, longer ones where that does not cover them
+struct Split {
+    int n_split, chunk;
+    float * o;                  // [n_split][n_rows][heads][hd] partial sums
+    float2 * ml;                // [n_split][n_rows][heads] (maximum, sum)
+    __host__ __device__ int span(int len) const {
+        const int even = (len + n_split - 1) / n_split;
+        return even <= chunk ? chunk : (even + 127) & ~127;
+    }
+    __host__ __device__ int used(int len) const { return len > 0 ? (len + span(len) - 1) / span(len) : 0; }
+};
+
+// What a CTA needs to know of its request: rows [row0, row1) of q, keys [0, len) of the table.
+struct Req {
+    int row0, row1, last, len, lens;
+};
+__device__ __forceinline__ Req request_of(const Kv4Attn & a, int page_shift, int r) {
+    Req q;
+    q.last = a.q_start[r + 1];
+    q.row0 = max(0, a.q_start[r]);
+    q.row1 = min(q.last, a.n_rows);
+    q.lens = a.lens[r];
+    q.len = (int) min((long long) max(q.lens, 0), (long long) a.width << page_shift);
+    return q;
+}
+// keys that row `row` sees
+__device__ __forceinline__ int visible(const Req & q, int row, int frame) {
+    if (frame == 0) return q.len;
+    const int p = q.lens - q.last + row;
+    if (p < 0) return 0;
+    const long long lim = ((long long) p / frame + 1) * frame;
+    return lim < q.len ? (int) lim : q.len;
+}
+
+__device__ __forceinline__ uint32_t smem_addr(const void * p) { return (uint32_t) __cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void * src, bool valid) {
+    const int n = valid ? 16 : 0;   // src-size 0 zero-fills the 16 bytes
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *(const uint32_t *) &h;
+}
+__device__ __forceinline__ uint32_t h2u(__half2 h) { return *(const uint32_t *) &h; }
+__device__ __forceinline__ __half2 u2h(uint32_t u) { return *(const __half2 *) &u; }
+
+// The nibbles 0 .. 3 of both 16-bit halves of u as four half2 of the integers -8 .. 7: 0x6400 | c is 1024 + c in f16,
+// 0x6400 | 16 c is 1024 + 16 c; both steps are exact.
+__device__ __forceinline__ uint32_t and_or(uint32_t u, uint32_t mask) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(u), "r"(mask), "r"(0x64006400u));
+    return r;
+}
+__device__ __forceinline__ void codes4(uint32_t u, __half2 (&x)[4]) {
+    const __half2 bias = u2h(0xe408e408u), sixteenth = u2h(0x2c002c00u), bias16 = u2h(0xd480d480u);   // -1032, 1/16, -72
+    const uint32_t v = u >> 8;
+    x[0] = __hadd2(u2h(and_or(u, 0x000f000fu)), bias);
+    x[1] = __hfma2(u2h(and_or(u, 0x00f000f0u)), sixteenth, bias16);
+    x[2] = __hadd2(u2h(and_or(v, 0x000f000fu)), bias);
+    x[3] = __hfma2(u2h(and_or(v, 0x00f000f0u)), sixteenth, bias16);
+}
+
+constexpr int STEP = 32;        // keys a warp takes at a time
+constexpr int STAGES = 3;
+constexpr int WARPS = 4;
+
+template <int NG> __host__ __device__ constexpr int row_bytes() { return 16 * NG; }
+template <int NG> __host__ __device__ constexpr int stage_bytes() { return 2 * STEP * row_bytes<NG>() + 2 * NG * STEP * 2; }
+template <int NG, int NT> constexpr int rows_smem() {
+    const int ring = WARPS * STAGES * stage_bytes<NG>(), merge = WARPS * 8 * NT * (32 * NG + 4 + 2) * 4;
+    return ring > merge ? ring : merge;
+}
+
+// Where row r of a step lies in a stage, and the 16-byte chunk c of it: rows 4 .. 7 of each 8 change places pairwise, and
+// of four-chunk rows every other pair swaps its halves, so that the reads below (8 lanes of consecutive rows, and 4
+// lanes of every other row) touch different banks.
+__device__ __forceinline__ int row_pos(int r) { return r ^ ((r >> 2) & 1); }
+template <int NG> __device__ __forceinline__ int chunk_pos(int pos, int c) { return NG == 4 ? c ^ (pos & 2) : c; }
+
+template <class T, int NG, int NT>
+__global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const Kv4Pool pool, const Kv4Attn a, const Split sp, int tiles,
+                                                                          int vec) {
+    constexpr int HD = 32 * NG, RB = row_bytes<NG>(), SB = stage_bytes<NG>(), MT = 2 * NG;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int h = blockIdx.y, r = blockIdx.z, kh = h / (a.heads / pool.heads);
-    const int q0 = max(0, a.q_start[r]), n = min(a.q_start[r + 1], a.n_rows) - q0;
-    const int P = 1 << pool.page_shift;
-    const int len = (int) min((long long) max(a.lens[r], 0), (long long) a.width << pool.page_shift);
-    const long long pages = pool.n_slots >> pool.page_shift;
-    for (int i = blockIdx.x * 4 + warp; i < n; i += gridDim.x * 4) {
-        const int keys = visible(a.lens[r] - n + i, len, a.frame);
-        float q[NG], acc[NG];
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ uint32_t s_poison[8 * NT];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int kh = blockIdx.y / tiles, r = blockIdx.z, G = a.heads / pool.heads;
+    const Req rq = request_of(a, pool.page_shift, r);
+    const int n_cols = (rq.row1 - rq.row0) * G;              // (token, head of the group) columns of this cache head
+    const int span = sp.span(rq.len), used = sp.used(rq.len);
+    const int k0 = blockIdx.x * span, k1 = min(rq.len, k0 + span);
+    if (n_cols <= 0 || (blockIdx.x && (int) blockIdx.x >= used)) return;
+    const int32_t * table = a.table + (size_t) r * a.width;
+    const int n_pages = (int) (pool.n_slots >> pool.page_shift), pmask = (1 << pool.page_shift) - 1;
+    uint8_t * ring = smem + warp * STAGES * SB;
+    const size_t plane = (size_t) pool.heads << pool.page_shift;     // rows of one plane of a page
+
+    for (int c0 = (int) (blockIdx.y % tiles) * 8 * NT; c0 < n_cols; c0 += tiles * 8 * NT) {
+        if (threadIdx.x < 8 * NT) s_poison[threadIdx.x] = 0;
+        // ---- the tile's columns: lane (g, t) loads channels 32 i + 8 t .. + 7 of column g of each 8
+        uint32_t qf[NT][NG][4];
+        float sl2[NT][2];
+        int lim[NT][2], low = 0x7fffffff;
 #pragma unroll
-        for (int g = 0; g < NG; g++) {
-            q[g] = from_type(((const T *) a.q)[(long long) (q0 + i) * a.q_tok + h * a.q_head + 32 * g + lane]);
-            acc[g] = 0.0f;
-        }
-        float m = -INFINITY, l = 0.0f;
-        for (int j = 0; j < keys; j++) {
-            const int page = a.table[(size_t) r * a.width + (j >> pool.page_shift)];
-            if (page < 0 || page >= pages) continue;
-            const int row = j & (P - 1);
-            const uint8_t * kq = pool.q + kv4_q_at(pool, page, 0, kh, row), * vq = pool.q + kv4_q_at(pool, page, 1, kh, row);
-            const __half * kd = pool.d + kv4_d_at(pool, page, 0, kh, row), * vd = pool.d + kv4_d_at(pool, page, 1, kh, row);
-            float s = 0.0f;
+        for (int nt = 0; nt < NT; nt++) {
+            const int col = c0 + 8 * nt + g;
+            const int row = rq.row0 + col / G, head = kh * G + col % G;
+            const T * q = (const T *) a.q + (long long) row * a.q_tok + head * a.q_head + 8 * t;
+            float amax = 0.0f, x[NG][8];
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const uint32_t b = kq[((lane >> 3) * NG + g) * 4 + ((lane & 7) >> 1)];
-                s += q[g] * ((float) ((int) ((b >> (4 * (lane & 1))) & 15u) - 8) * __half2float(kd[(size_t) g * P]));
+            for (int i = 0; i < NG; i++) {
+                T e[8];
+                if (col >= n_cols) {
+#pragma unroll
+                    for (int c = 0; c < 8; c++) e[c] = to_type<T>(0.0f);
+                } else if (vec & 1) {
+                    *(uint4 *) e = *(const uint4 *) (q + 32 * i);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 8; c++) e[c] = q[32 * i + c];
+                }
+#pragma unroll
+                for (int c = 0; c < 8; c++) { x[i][c] = from_type(e[c]); amax = fmaxf(amax, fabsf(x[i][c])); }
             }
+            int ex = 0;                                      // the row is multiplied by 2^ex
+            if (!std::is_same<T, __half>::value) {
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                const int e = (int) (__float_as_uint(amax) >> 23);     // biased exponent; 255: not finite
+                if (amax > 0.0f && e < 255) ex = min(14 - (e - 127), 126);
+            }
+            const float up = __int_as_float((127 + ex) << 23);
 #pragma unroll
-            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            s *= a.scale;
-            const float nm = fmaxf(m, s), c = m == nm ? 1.0f : expf(m - nm), w = s == nm ? 1.0f : expf(s - nm);
-            m = nm;
-            l = l * c + w;
+            for (int i = 0; i < NG; i++) {
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const uint32_t b = vq[16 * g + (lane >> 1)];
-                acc[g] = acc[g] * c + w * ((float) ((int) ((b >> (4 * (lane & 1))) & 15u) - 8) * __half2float(vd[(size_t) g * P]));
+                for (int c = 0; c < 4; c++) qf[nt][i][c] = pack_h2(x[i][c] * up, x[i][c + 4] * up);
+            }
+            // the factor of the scores of columns 2 t and 2 t + 1 (in log2 units), and the keys they see
+            const float f = a.scale * 1.4426950408889634f * __int_as_float((127 - ex) << 23);
+            const int see = col < n_cols ? visible(rq, row, a.frame) : 0x7fffffff;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                sl2[nt][e] = __shfl_sync(0xffffffffu, f, 4 * (2 * t + e));
+                lim[nt][e] = __shfl_sync(0xffffffffu, see, 4 * (2 * t + e));
+                low = min(low, lim[nt][e]);
             }
         }
-        const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+        low = min(low, __shfl_xor_sync(0xffffffffu, low, 1));
+        low = min(low, __shfl_xor_sync(0xffffffffu, low, 2));
+
+        float o[MT][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
-        for (int g = 0; g < NG; g++) {
-            ((T *) a.out)[(long long) (q0 + i) * a.o_tok + h * a.o_head + 32 * g + lane] = to_type<T>(acc[g] * inv);
+        for (int nt = 0; nt < NT; nt++) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < MT; i++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
         }
+        __syncthreads();                                     // s_poison is clear
+
+        // ---- the ring: step i of this warp holds keys k0 + 32 (4 i + warp) ..; a step touches two pages at most
+        const int steps = (max(0, k1 - k0) + STEP - 1) / STEP, mine = steps > warp ? (steps - warp + WARPS - 1) / WARPS : 0;
+        auto page_at = [&](int key) -> int {
+            const int i = key >> pool.page_shift;
+            const int p = i < a.width && key < k1 ? __ldg(table + i) : -1;
+            return p < n_pages ? p : -1;
+        };
+        int pg0 = -1, pg1 = -1;                              // the pages of the next step to be issued
+        if (mine) { const int key = k0 + STEP * warp; pg0 = page_at(key); pg1 = page_at(key + 16); }
+        uint32_t holes = 0;                                  // 2 bits a stage: halves of the step that have no page
+        auto issue = [&](int i) {
+            if (i < mine) {
+                const int key = k0 + STEP * (WARPS * i + warp), s = i % STAGES;
+                const uint32_t base = smem_addr(ring + s * SB);
+                const size_t row0 = (((size_t) max(pg0, 0) * 2 * pool.heads + kh) << pool.page_shift) + (key & pmask);
+                const size_t row1 = (((size_t) max(pg1, 0) * 2 * pool.heads + kh) << pool.page_shift) + ((key + 16) & pmask);
+#pragma unroll
+                for (int e = lane; e < STEP * NG; e += 32) {
+                    const int rr = e / NG, c = e % NG, pos = row_pos(rr);
+                    const size_t row = rr < 16 ? row0 + rr : row1 + rr - 16;
+                    const bool ok = (rr < 16 ? pg0 : pg1) >= 0;
+                    const uint8_t * src = pool.q + row * RB + 16 * c;
+                    const uint32_t dst = base + pos * RB + 16 * chunk_pos<NG>(pos, c);
+                    cp_async16(dst, src, ok);
+                    cp_async16(dst + STEP * RB, src + plane * RB, ok);
+                }
+                if (lane < 8 * NG) {                         // 8 scales at a time: (plane, group, quarter of the step)
+                    const int pl = lane / (4 * NG), grp = (lane / 4) % NG, qt = lane & 3;
+                    const int pg = qt < 2 ? pg0 : pg1;
+                    const size_t at = kv4_d_at(pool, max(pg, 0), pl, kh, (key + 8 * qt) & pmask) + ((size_t) grp << pool.page_shift);
+                    cp_async16(base + 2 * STEP * RB + ((pl * NG + grp) * STEP + 8 * qt) * 2, pool.d + at, pg >= 0);
+                }
+                holes = (holes & ~(3u << (2 * s))) | (((pg0 < 0 ? 1u : 0u) | (pg1 < 0 ? 2u : 0u)) << (2 * s));
+                if (i + 1 < mine) { const int next = key + STEP * WARPS; pg0 = page_at(next); pg1 = page_at(next + 16); }
+            }
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; i++) issue(i);
+
+        for (int i = 0; i < mine; i++) {
+            cp_async_wait<STAGES - 2>();
+            __syncwarp();                                    // everyone's copies of step i are in, and step i - 1 is read
+            const int st = i % STAGES;
+            const uint32_t hole = (holes >> (2 * st)) & 3u;
+            issue(i + STAGES - 1);
+            const uint8_t * kb = ring + st * SB, * vb = kb + STEP * RB;
+            const __half * kd = (const __half *) (vb + STEP * RB), * vd = kd + NG * STEP;
+            const int key = k0 + STEP * (WARPS * i + warp);
+            // ---- scores
+            float s[2][NT][4];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                uint32_t w[2][NG];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int pos = row_pos(16 * u + 8 * h + g);
+                    const uint8_t * p = kb + pos * RB;
+                    if (NG == 4) {
+                        const uint4 x = *(const uint4 *) (p + 16 * chunk_pos<NG>(pos, t));
+                        w[h][0] = x.x; w[h][1 % NG] = x.y; w[h][2 % NG] = x.z; w[h][3 % NG] = x.w;
+                    } else if (NG == 2) {
+                        const uint2 x = *(const uint2 *) (p + 8 * t);
+                        w[h][0] = x.x; w[h][1 % NG] = x.y;
+                    } else {
+#pragma unroll
+                        for (int gi = 0; gi < NG; gi++) w[h][gi] = *(const uint32_t *) (p + 4 * (t * NG + gi));
+                    }
+                }
+#pragma unroll
+                for (int gi = 0; gi < NG; gi++) {
+                    __half2 x0[4], x1[4];
+                    codes4(w[0][gi], x0);
+                    codes4(w[1][gi], x1);
+                    const float d0 = __half2float(kd[gi * STEP + 16 * u + g]), d1 = __half2float(kd[gi * STEP + 16 * u + 8 + g]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        mma16816(acc, {h2u(x0[0]), h2u(x1[0]), h2u(x0[1]), h2u(x1[1])}, qf[nt][gi][0], qf[nt][gi][1]);
+                        mma16816(acc, {h2u(x0[2]), h2u(x1[2]), h2u(x0[3]), h2u(x1[3])}, qf[nt][gi][2], qf[nt][gi][3]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float d = e < 2 ? d0 : d1;
+                            s[u][nt][e] = gi == 0 ? d * acc[e] : __fmaf_rn(d, acc[e], s[u][nt][e]);
+                        }
+                    }
+                }
+            }
+            const bool whole = key + STEP <= min(low, k1) && hole == 0;
+            float mx[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                mx[nt][0] = mx[nt][1] = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        float x = s[u][nt][e] * sl2[nt][e & 1];
+                        if (!whole) {
+                            const int k = key + 16 * u + 8 * (e >> 1) + g;
+                            if (k >= min(lim[nt][e & 1], k1) || ((hole >> u) & 1)) x = -INFINITY;
+                        }
+                        s[u][nt][e] = x;
+                        mx[nt][e & 1] = fmaxf(mx[nt][e & 1], x);
+                    }
+                }
+            }
+            bool raise = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) raise = raise || mx[nt][0] > m[nt][0] + 4.0f || mx[nt][1] > m[nt][1] + 4.0f;
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float x = mx[nt][e];
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                        x = fmaxf(x, m[nt][e]);
+                        const float c = x == m[nt][e] ? 1.0f : ex2(m[nt][e] - x);
+                        m[nt][e] = x;
+                        l[nt][e] *= c;
+#pragma unroll
+                        for (int k = 0; k < MT; k++) { o[k][nt][e] *= c; o[k][nt][e + 2] *= c; }
+                    }
+                }
+            }
+            // ---- weights, as the B operand of the second product
+            uint32_t pf[2][NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                const float z0 = (m[nt][0] == -INFINITY ? 0.0f : m[nt][0]) - 10.0f, z1 = (m[nt][1] == -INFINITY ? 0.0f : m[nt][1]) - 10.0f;
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const float p0 = ex2(s[u][nt][0] - z0), p1 = ex2(s[u][nt][1] - z1), p2 = ex2(s[u][nt][2] - z0), p3 = ex2(s[u][nt][3] - z1);
+                    l[nt][0] += p0 + p2;
+                    l[nt][1] += p1 + p3;
+                    pf[u][nt][0] = transpose8(pack_h2(p0, p1));
+                    pf[u][nt][1] = transpose8(pack_h2(p2, p3));
+                }
+            }
+            // ---- sums of values
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int ra = 16 * u + 2 * t;                         // this lane's keys: ra, ra + 1, ra + 8, ra + 9
+                constexpr int PARTS = NG % 2 ? NG : NG / 2;           // 32 or 64 channels at a time
+#pragma unroll
+                for (int j = 0; j < PARTS; j++) {
+                    const int grp = NG % 2 ? j : 2 * j + (g >> 2);
+                    __half2 d0 = *(const __half2 *) (vd + grp * STEP + ra), d1 = *(const __half2 *) (vd + grp * STEP + ra + 8);
+                    if (!whole) {
+                        // a weight of 0 does not silence a value that is not a number: such scales become 0 here, and the
+                        // columns that see the key get their NaN at the end
+                        const __half e[4] = {__low2half(d0), __high2half(d0), __low2half(d1), __high2half(d1)};
+                        __half f[4];
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            f[c] = e[c];
+                            if (__hisnan(e[c]) || __hisinf(e[c])) {
+                                f[c] = __ushort_as_half(0);
+                                const int k = key + ra + (c & 1) + 8 * (c >> 1);
+                                for (int col = 0; col < 8 * NT; col++) {
+                                    const int cc = c0 + col;
+                                    if (cc < n_cols && k < k1 && k < visible(rq, rq.row0 + cc / G, a.frame)) atomicOr(&s_poison[col], 1u << grp);
+                                }
+                            }
+                        }
+                        d0 = __halves2half2(f[0], f[1]);
+                        d1 = __halves2half2(f[2], f[3]);
+                    }
+                    uint32_t w[4];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const int pos = row_pos(ra + (c & 1) + 8 * (c >> 1));
+                        if (NG % 2) w[c] = *(const uint16_t *) (vb + pos * RB + 16 * j + 2 * g);
+                        else w[c] = *(const uint32_t *) (vb + pos * RB + 16 * chunk_pos<NG>(pos, 2 * j + (g >> 2)) + 4 * (g & 3));
+                    }
+#pragma unroll
+                    for (int h = 0; h < (NG % 2 ? 1 : 2); h++) {
+                        const uint32_t sel = h ? 0x7632 : 0x5410;      // half h of one key's word beside the next key's
+                        __half2 x[4], y[4];
+                        codes4(__byte_perm(w[0], w[1], sel), x);
+                        codes4(__byte_perm(w[2], w[3], sel), y);
+#pragma unroll
+                        for (int c = 0; c < 4; c++) { x[c] = __hmul2(x[c], d0); y[c] = __hmul2(y[c], d1); }
+                        const int mt = NG % 2 ? 2 * j : 4 * j + 2 * h;
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            mma16816(o[mt][nt], {h2u(x[0]), h2u(x[1]), h2u(y[0]), h2u(y[1])}, pf[u][nt][0], pf[u][nt][1]);
+                            mma16816(o[mt + 1][nt], {h2u(x[2]), h2u(x[3]), h2u(y[2]), h2u(y[3])}, pf[u][nt][0], pf[u][nt][1]);
+                        }
+                    }
+                }
+            }
+        }
+        cp_async_wait<0>();
+        __syncthreads();                                     // the rings become the merge's buffers
+
+        // ---- merge the four warps: [warp][column][hd + 4], then (maximum, sum) [warp][column]
+        float * so = (float *) smem;
+        float2 * sm = (float2 *) (so + WARPS * 8 * NT * (HD + 4));
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float x = l[nt][e];
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+                const int col = warp * 8 * NT + 8 * nt + 2 * t + e;
+                if (g == 0) sm[col] = make_float2(m[nt][e], x);
+#pragma unroll
+                for (int k = 0; k < MT; k++) {
+                    const int c = NG % 2 ? 32 * (k / 2) + 4 * g + 2 * (k % 2) : 64 * (k / 4) + 8 * g + 2 * (k % 4);
+                    *(float2 *) (so + col * (HD + 4) + c) = make_float2(o[k][nt][e], o[k][nt][e + 2]);
+                }
+            }
+        }
+        __syncthreads();
+        for (int idx = threadIdx.x; idx < 8 * NT * (HD / 4); idx += 32 * WARPS) {
+            const int col = idx / (HD / 4), c = idx % (HD / 4) * 4;
+            if (c0 + col >= n_cols) continue;
+            float top = -INFINITY, sum = 0.0f;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) top = fmaxf(top, sm[w * 8 * NT + col].x);
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) {
+                const float2 ml = sm[w * 8 * NT + col];
+                const float f = ml.x == -INFINITY ? 0.0f : ml.x == top ? 1.0f : ex2(ml.x - top);
+                const float4 x = *(const float4 *) (so + (w * 8 * NT + col) * (HD + 4) + c);
+                // a warp that saw nothing holds zeros, or what a score that is not a number has made of them
+                const float k = ml.x == -INFINITY ? 1.0f : f;
+                sum = __fmaf_rn(ml.y, k, sum);
+                v.x = __fmaf_rn(x.x, k, v.x); v.y = __fmaf_rn(x.y, k, v.y); v.z = __fmaf_rn(x.z, k, v.z); v.w = __fmaf_rn(x.w, k, v.w);
+            }
+            if ((s_poison[col] >> (c / 32)) & 1) v.x = v.y = v.z = v.w = __int_as_float(0x7fffffff);
+            const int row = rq.row0 + (c0 + col) / G, head = kh * G + (c0 + col) % G;
+            if (used <= 1) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                T * out = (T *) a.out + (long long) row * a.o_tok + head * a.o_head + c;
+                const T y[4] = {to_type<T>(v.x * inv), to_type<T>(v.y * inv), to_type<T>(v.z * inv), to_type<T>(v.w * inv)};
+                if (vec & 2) {
+                    uint2 w;
+                    memcpy(&w, y, 8);
+                    *(uint2 *) out = w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) out[e] = y[e];
+                }
+            } else {
+                const size_t at = ((size_t) blockIdx.x * a.n_rows + row) * a.heads + head;
+                *(float4 *) (sp.o + at * HD + c) = v;
+                if (c == 0) sp.ml[at] = make_float2(top, sum);
+            }
+        }
+        __syncthreads();
     }
 }
 
-template <class T>
+// Joins the partial sums of a row: one CTA per (row, head), its warps taking every eighth part.
+template <class T, int NG>
+__global__ void __launch_bounds__(256) k_kv4_merge(const Kv4Pool pool, const Kv4Attn a, const Split sp) {
+    constexpr int HD = 32 * NG;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ float s_top[8], s_sum[8], s_o[8][HD];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y;
+    const Req rq = request_of(a, pool.page_shift, blockIdx.z);
+    const int used = sp.used(rq.len);
+    if (used <= 1) return;                                   // written by the first kernel
+    for (int row = rq.row0 + blockIdx.x; row < rq.row1; row += gridDim.x) {
+        const size_t at = (size_t) row * a.heads + head, step = (size_t) a.n_rows * a.heads;
+        float top = -INFINITY;
+        for (int s = threadIdx.x; s < used; s += 256) top = fmaxf(top, sp.ml[at + s * step].x);
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        if (lane == 0) s_top[warp] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 8; w++) top = fmaxf(top, s_top[w]);
+        float sum = 0.0f, v[NG];
+#pragma unroll
+        for (int i = 0; i < NG; i++) v[i] = 0.0f;
+#pragma unroll 4
+        for (int s = warp; s < used; s += 8) {
+            const float2 ml = sp.ml[at + s * step];
+            const float f = ml.x == top || ml.x == -INFINITY ? 1.0f : ex2(ml.x - top);   // -inf: zeros, or NaN to be kept
+            sum = __fmaf_rn(ml.y, f, sum);
+#pragma unroll
+            for (int i = 0; i < NG; i++) v[i] = __fmaf_rn(sp.o[(at + s * step) * HD + 32 * i + lane], f, v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NG; i++) s_o[warp][32 * i + lane] = v[i];
+        if (lane == 0) s_sum[warp] = sum;
+        __syncthreads();
+        for (int c = threadIdx.x; c < HD; c += 256) {
+            float x = 0.0f, z = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 8; w++) { x += s_o[w][c]; z += s_sum[w]; }
+            ((T *) a.out)[(long long) row * a.o_tok + head * a.o_head + c] = to_type<T>(z == 0.0f ? x * 0.0f : x / z);
+        }
+        __syncthreads();
+    }
+}
+
+// The launch of the rows kernel: columns a CTA takes, CTAs along the columns, and the division of the keys.
+struct RowsPlan {
+    int nt, tiles;
+    Split sp;
+};
+RowsPlan rows_plan(const Kv4Pool & p, const Kv4Attn & a) {
+    RowsPlan r;
+    const long long cols = (long long) a.max_new * (a.heads / p.heads);
+    r.nt = cols > 8 ? 2 : 1;
+    r.tiles = (int) std::min<long long>((cols + 8 * r.nt - 1) / (8 * r.nt), 65535 / p.heads);
+    // about 148 SMs x 4 CTAs x 3 ranges of equal length if every request is as long as the longest; 256 keys at least
+    const long long total = (long long) a.n_req * p.heads * r.tiles * a.max_len;
+    const long long chunk = std::max<long long>(256, (total / (148 * 4 * 3) + 127) & ~127LL);
+    r.sp.chunk = (int) std::min<long long>(chunk, 0x7fffff00);
+    r.sp.n_split = (a.max_len + r.sp.chunk - 1) / r.sp.chunk;
+    r.sp.o = nullptr;
+    r.sp.ml = nullptr;
+    return r;
+}
+
+size_t partial_bytes(const Kv4Pool & p, const Kv4Attn & a, int n_split) {
+    return n_split <= 1 ? 0 : (size_t) n_split * a.n_rows * a.heads * (p.hd + 2) * 4;
+}
+
+template <class T, int NG, int NT>
+int rows_launch(const Kv4Pool & p, const Kv4Attn & a, RowsPlan r, int vec, cudaStream_t st) {
+    constexpr int smem = rows_smem<NG, NT>();
+    JB_CUDA(cudaFuncSetAttribute(k_kv4_rows<T, NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    const dim3 grid((unsigned) r.sp.n_split, (unsigned) (p.heads * r.tiles), (unsigned) a.n_req);
+    JB_CUDA(launch_pdl(k_kv4_rows<T, NG, NT>, grid, dim3(32 * WARPS), smem, st, p, a, r.sp, r.tiles, vec));
+    return 0;
+}
+
+template <class T, int NG>
 int launch(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st) {
-    const dim3 grid((unsigned) ((a.max_new + 3) / 4), (unsigned) a.heads, (unsigned) a.n_req);
-    switch (p.hd / 32) {
-        case 1: JB_CUDA(launch_pdl(k_kv4_attention<T, 1>, grid, dim3(128), 0, st, p, a)); break;
-        case 2: JB_CUDA(launch_pdl(k_kv4_attention<T, 2>, grid, dim3(128), 0, st, p, a)); break;
-        case 3: JB_CUDA(launch_pdl(k_kv4_attention<T, 3>, grid, dim3(128), 0, st, p, a)); break;
-        default: JB_CUDA(launch_pdl(k_kv4_attention<T, 4>, grid, dim3(128), 0, st, p, a)); break;
+    RowsPlan r = rows_plan(p, a);
+    if (r.sp.n_split > 1) {
+        r.sp.o = (float *) a.ws;
+        r.sp.ml = (float2 *) (r.sp.o + (size_t) r.sp.n_split * a.n_rows * a.heads * p.hd);
+    }
+    // 16-byte loads of q, 8-byte stores of out where the strides allow them
+    const int vec = (((uintptr_t) a.q & 15) == 0 && ((a.q_tok | a.q_head) & 7) == 0 ? 1 : 0) |
+                    (((uintptr_t) a.out & 7) == 0 && ((a.o_tok | a.o_head) & 3) == 0 ? 2 : 0);
+    if (r.nt == 1 ? rows_launch<T, NG, 1>(p, a, r, vec, st) : rows_launch<T, NG, 2>(p, a, r, vec, st)) return -1;
+    if (r.sp.n_split > 1) {
+        const dim3 grid((unsigned) std::max(1, a.max_new), (unsigned) a.heads, (unsigned) a.n_req);
+        JB_CUDA(launch_pdl(k_kv4_merge<T, NG>, grid, dim3(256), 0, st, p, a, r.sp));
     }
     return 0;
 }
 
+template <class T>
+int launch_dim(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st) {
+    switch (p.hd / 32) {
+        case 1: return launch<T, 1>(p, a, st);
+        case 2: return launch<T, 2>(p, a, st);
+        case 3: return launch<T, 3>(p, a, st);
+        default: return launch<T, 4>(p, a, st);
+    }
+}
+
 }  // namespace
 
-size_t kv4_attention_workspace(const Kv4Pool &, const Kv4Attn &) { return 0; }
+size_t kv4_attention_workspace(const Kv4Pool & p, const Kv4Attn & a) {
+    if (!a.n_req || !a.n_rows) return 0;
+    return partial_bytes(p, a, rows_plan(p, a).sp.n_split);
+}
 
 int kv4_attention(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st) {
     KTimer kt("kv4_attention", st);
-    return a.type == KV4_F16 ? launch<__half>(p, a, st) : launch<__nv_bfloat16>(p, a, st);
+    return a.type == KV4_F16 ? launch_dim<__half>(p, a, st) : launch_dim<__nv_bfloat16>(p, a, st);
 }
 
 }  // namespace jb
