@@ -28,6 +28,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 namespace jb {
@@ -81,9 +82,8 @@ __device__ __forceinline__ int visible(const Req & q, int row, int frame) {
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void * p) { return (uint32_t) __cvta_generic_to_shared(p); }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void * src, bool valid) {
-    const int n = valid ? 16 : 0;   // src-size 0 zero-fills the 16 bytes
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(n) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void * src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
@@ -93,6 +93,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  "{%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// d = a b
+__device__ __forceinline__ void mma16816_0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%10, %10, %10, %10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
@@ -147,6 +154,7 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ uint32_t s_poison[8 * NT];
+    __shared__ int2 s_col[8 * NT];                           // row and head of each column
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int kh = blockIdx.y / tiles, r = blockIdx.z, G = a.heads / pool.heads;
     const Req rq = request_of(a, pool.page_shift, r);
@@ -157,7 +165,21 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
     const int32_t * table = a.table + (size_t) r * a.width;
     const int n_pages = (int) (pool.n_slots >> pool.page_shift), pmask = (1 << pool.page_shift) - 1;
     uint8_t * ring = smem + warp * STAGES * SB;
-    const size_t plane = (size_t) pool.heads << pool.page_shift;     // rows of one plane of a page
+    // addresses of this cache head: bytes from page to page and from keys to values, this lane's scales (lane = (plane,
+    // group, quarter of a step), in the order in which a stage holds them) and its place among a copy's rows
+    const uint32_t q_plane = ((uint32_t) pool.heads << pool.page_shift) * RB, q_page = 2 * q_plane;   // at most 2^25 bytes
+    const uint8_t * q_head = pool.q + ((size_t) kh << pool.page_shift) * RB;
+    const uint32_t d_page = ((uint32_t) 2 * pool.heads * NG) << pool.page_shift;
+    const __half * d_lane = pool.d + ((((size_t) (lane / (4 * NG)) * pool.heads + kh) * NG + (lane / 4) % NG) << pool.page_shift) + 8 * (lane & 1);
+    const uint32_t ring_s = smem_addr(ring);
+    const uint32_t copy_dst = row_pos(lane / NG) * RB + 16 * chunk_pos<NG>(row_pos(lane / NG), lane % NG);
+    // where this lane reads: its words of key row g, and of the value rows 2 t and 2 t + 1 (NG odd: half-words)
+    const int k_at = row_pos(g) * RB + (NG == 4 ? 16 * chunk_pos<NG>(row_pos(g), t) : 4 * NG * t);
+    const int v_a = row_pos(2 * t), v_b = row_pos(2 * t + 1);
+    const int v_at[2] = {v_a * RB + (NG % 2 ? 2 * g : 16 * chunk_pos<NG>(v_a, g >> 2) + 4 * (g & 3)),
+                         v_b * RB + (NG % 2 ? 2 * g : 16 * chunk_pos<NG>(v_b, g >> 2) + 4 * (g & 3))};
+    // .. and from there to the second 64 channels (of four-chunk rows: the other two chunks, which side depends on the row)
+    const int v_step[2] = {NG == 4 && (v_a & 2) ? -32 : 32, NG == 4 && (v_b & 2) ? -32 : 32};
 
     for (int c0 = (int) (blockIdx.y % tiles) * 8 * NT; c0 < n_cols; c0 += tiles * 8 * NT) {
         if (threadIdx.x < 8 * NT) s_poison[threadIdx.x] = 0;
@@ -169,6 +191,7 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
         for (int nt = 0; nt < NT; nt++) {
             const int col = c0 + 8 * nt + g;
             const int row = rq.row0 + col / G, head = kh * G + col % G;
+            if (threadIdx.x < 32 && t == 0) s_col[8 * nt + g] = make_int2(row, head);
             const T * q = (const T *) a.q + (long long) row * a.q_tok + head * a.q_head + 8 * t;
             float amax = 0.0f, x[NG][8];
 #pragma unroll
@@ -187,12 +210,10 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
                 for (int c = 0; c < 8; c++) { x[i][c] = from_type(e[c]); amax = fmaxf(amax, fabsf(x[i][c])); }
             }
             int ex = 0;                                      // the row is multiplied by 2^ex
-            if (!std::is_same<T, __half>::value) {
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                const int e = (int) (__float_as_uint(amax) >> 23);     // biased exponent; 255: not finite
-                if (amax > 0.0f && e < 255) ex = min(14 - (e - 127), 126);
-            }
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            const int eb = (int) (__float_as_uint(amax) >> 23);        // biased exponent; 255: not finite
+            if (amax > 0.0f && eb < 255) ex = min(14 - (eb - 127), 126);
             const float up = __int_as_float((127 + ex) << 23);
 #pragma unroll
             for (int i = 0; i < NG; i++) {
@@ -212,10 +233,12 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
         low = min(low, __shfl_xor_sync(0xffffffffu, low, 1));
         low = min(low, __shfl_xor_sync(0xffffffffu, low, 2));
 
-        float o[MT][NT][4], m[NT][2], l[NT][2];
+        // z: the running maximum less 10; weights are 2^(s - z). Before the first score: the lowest float, below which no
+        // finite score lies
+        float o[MT][NT][4], z[NT][2], l[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            m[nt][0] = m[nt][1] = -INFINITY;
+            z[nt][0] = z[nt][1] = -FLT_MAX;
             l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
             for (int i = 0; i < MT; i++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
@@ -231,30 +254,33 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
         };
         int pg0 = -1, pg1 = -1;                              // the pages of the next step to be issued
         if (mine) { const int key = k0 + STEP * warp; pg0 = page_at(key); pg1 = page_at(key + 16); }
-        uint32_t holes = 0;                                  // 2 bits a stage: halves of the step that have no page
+        uint32_t holes = 0;                                  // 2 bits a step, the oldest lowest: halves that have no page
+        uint32_t fill = 0, read = 0;                         // byte offsets of the stage to be filled and read next
         auto issue = [&](int i) {
             if (i < mine) {
-                const int key = k0 + STEP * (WARPS * i + warp), s = i % STAGES;
-                const uint32_t base = smem_addr(ring + s * SB);
-                const size_t row0 = (((size_t) max(pg0, 0) * 2 * pool.heads + kh) << pool.page_shift) + (key & pmask);
-                const size_t row1 = (((size_t) max(pg1, 0) * 2 * pool.heads + kh) << pool.page_shift) + ((key + 16) & pmask);
+                // a half without a page copies page 0's rows, which are masked
+                const int key = k0 + STEP * (WARPS * i + warp);
+                const uint32_t dst = ring_s + fill;
+                fill = fill == (STAGES - 1) * SB ? 0 : fill + SB;
+                const uint8_t * src[2] = {q_head + (uint64_t) (uint32_t) max(pg0, 0) * q_page + (key & pmask) * RB,
+                                          q_head + (uint64_t) (uint32_t) max(pg1, 0) * q_page + ((key + 16) & pmask) * RB};
 #pragma unroll
-                for (int e = lane; e < STEP * NG; e += 32) {
-                    const int rr = e / NG, c = e % NG, pos = row_pos(rr);
-                    const size_t row = rr < 16 ? row0 + rr : row1 + rr - 16;
-                    const bool ok = (rr < 16 ? pg0 : pg1) >= 0;
-                    const uint8_t * src = pool.q + row * RB + 16 * c;
-                    const uint32_t dst = base + pos * RB + 16 * chunk_pos<NG>(pos, c);
-                    cp_async16(dst, src, ok);
-                    cp_async16(dst + STEP * RB, src + plane * RB, ok);
+                for (int e = 0; e < NG; e++) {               // 8 rows of 4 chunks (NG 4), 16 of 2, 32 of 1; NG 3: 32 chunks
+                    const int c = lane + 32 * e, rr = c / NG, pos = row_pos(rr);
+                    const uint8_t * x = NG == 3 ? (rr < 16 ? src[0] : src[1]) + (rr & 15) * RB + 16 * (c % NG)
+                                     : NG == 1 ? (lane < 16 ? src[0] : src[1]) + (lane & 15) * 16
+                                               : src[e * 32 / NG / 16] + lane * 16 + ((e * 32 / NG) & 15) * RB;
+                    const uint32_t y = NG == 4 ? copy_dst + e * 8 * RB : NG == 2 ? copy_dst + e * 16 * RB
+                                     : pos * RB + 16 * chunk_pos<NG>(pos, c % NG);
+                    cp_async16(dst + y, x);
+                    cp_async16(dst + y + STEP * RB, x + q_plane);
                 }
                 if (lane < 8 * NG) {                         // 8 scales at a time: (plane, group, quarter of the step)
-                    const int pl = lane / (4 * NG), grp = (lane / 4) % NG, qt = lane & 3;
-                    const int pg = qt < 2 ? pg0 : pg1;
-                    const size_t at = kv4_d_at(pool, max(pg, 0), pl, kh, (key + 8 * qt) & pmask) + ((size_t) grp << pool.page_shift);
-                    cp_async16(base + 2 * STEP * RB + ((pl * NG + grp) * STEP + 8 * qt) * 2, pool.d + at, pg >= 0);
+                    const __half * x = (lane & 2 ? d_lane + (uint64_t) (uint32_t) max(pg1, 0) * d_page + ((key + 16) & pmask)
+                                                 : d_lane + (uint64_t) (uint32_t) max(pg0, 0) * d_page + (key & pmask));
+                    cp_async16(dst + 2 * STEP * RB + 16 * lane, x);
                 }
-                holes = (holes & ~(3u << (2 * s))) | (((pg0 < 0 ? 1u : 0u) | (pg1 < 0 ? 2u : 0u)) << (2 * s));
+                holes |= ((uint32_t) pg0 >> 31 | (uint32_t) pg1 >> 31 << 1) << (2 * (i < STAGES - 1 ? i : STAGES - 1));
                 if (i + 1 < mine) { const int next = key + STEP * WARPS; pg0 = page_at(next); pg1 = page_at(next + 16); }
             }
             cp_async_commit();
@@ -265,10 +291,11 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
         for (int i = 0; i < mine; i++) {
             cp_async_wait<STAGES - 2>();
             __syncwarp();                                    // everyone's copies of step i are in, and step i - 1 is read
-            const int st = i % STAGES;
-            const uint32_t hole = (holes >> (2 * st)) & 3u;
             issue(i + STAGES - 1);
-            const uint8_t * kb = ring + st * SB, * vb = kb + STEP * RB;
+            const uint32_t hole = holes & 3u;
+            holes >>= 2;
+            const uint8_t * kb = ring + read, * vb = kb + STEP * RB;
+            read = read == (STAGES - 1) * SB ? 0 : read + SB;
             const __half * kd = (const __half *) (vb + STEP * RB), * vd = kd + NG * STEP;
             const int key = k0 + STEP * (WARPS * i + warp);
             // ---- scores
@@ -278,17 +305,16 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
                 uint32_t w[2][NG];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const int pos = row_pos(16 * u + 8 * h + g);
-                    const uint8_t * p = kb + pos * RB;
+                    const uint8_t * p = kb + k_at + (16 * u + 8 * h) * RB;
                     if (NG == 4) {
-                        const uint4 x = *(const uint4 *) (p + 16 * chunk_pos<NG>(pos, t));
+                        const uint4 x = *(const uint4 *) p;
                         w[h][0] = x.x; w[h][1 % NG] = x.y; w[h][2 % NG] = x.z; w[h][3 % NG] = x.w;
                     } else if (NG == 2) {
-                        const uint2 x = *(const uint2 *) (p + 8 * t);
+                        const uint2 x = *(const uint2 *) p;
                         w[h][0] = x.x; w[h][1 % NG] = x.y;
                     } else {
 #pragma unroll
-                        for (int gi = 0; gi < NG; gi++) w[h][gi] = *(const uint32_t *) (p + 4 * (t * NG + gi));
+                        for (int gi = 0; gi < NG; gi++) w[h][gi] = *(const uint32_t *) (p + 4 * gi);
                     }
                 }
 #pragma unroll
@@ -299,8 +325,8 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
                     const float d0 = __half2float(kd[gi * STEP + 16 * u + g]), d1 = __half2float(kd[gi * STEP + 16 * u + 8 + g]);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        mma16816(acc, {h2u(x0[0]), h2u(x1[0]), h2u(x0[1]), h2u(x1[1])}, qf[nt][gi][0], qf[nt][gi][1]);
+                        float acc[4];
+                        mma16816_0(acc, {h2u(x0[0]), h2u(x1[0]), h2u(x0[1]), h2u(x1[1])}, qf[nt][gi][0], qf[nt][gi][1]);
                         mma16816(acc, {h2u(x0[2]), h2u(x1[2]), h2u(x0[3]), h2u(x1[3])}, qf[nt][gi][2], qf[nt][gi][3]);
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
@@ -311,27 +337,38 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
                 }
             }
             const bool whole = key + STEP <= min(low, k1) && hole == 0;
-            float mx[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                mx[nt][0] = mx[nt][1] = -INFINITY;
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        float x = s[u][nt][e] * sl2[nt][e & 1];
-                        if (!whole) {
-                            const int k = key + 16 * u + 8 * (e >> 1) + g;
-                            if (k >= min(lim[nt][e & 1], k1) || ((hole >> u) & 1)) x = -INFINITY;
-                        }
-                        s[u][nt][e] = x;
-                        mx[nt][e & 1] = fmaxf(mx[nt][e & 1], x);
-                    }
+                    for (int e = 0; e < 4; e++) s[u][nt][e] *= sl2[nt][e & 1];
                 }
             }
+            if (!whole) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int k = key + 16 * u + 8 * (e >> 1) + g;
+                            if (k >= min(lim[nt][e & 1], k1) || ((hole >> u) & 1)) s[u][nt][e] = -INFINITY;
+                        }
+                    }
+                }
+                asm volatile("" ::: "memory");               // a branch, not selects in every step
+            }
+            float mx[NT][2];
             bool raise = false;
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) raise = raise || mx[nt][0] > m[nt][0] + 4.0f || mx[nt][1] > m[nt][1] + 4.0f;
+            for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    mx[nt][e] = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
+                    raise = raise || mx[nt][e] > z[nt][e] + 14.0f;
+                }
+            }
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
@@ -340,9 +377,9 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
                         float x = mx[nt][e];
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                        x = fmaxf(x, m[nt][e]);
-                        const float c = x == m[nt][e] ? 1.0f : ex2(m[nt][e] - x);
-                        m[nt][e] = x;
+                        x = fmaxf(x - 10.0f, z[nt][e]);
+                        const float c = x == z[nt][e] ? 1.0f : ex2(z[nt][e] - x);
+                        z[nt][e] = x;
                         l[nt][e] *= c;
 #pragma unroll
                         for (int k = 0; k < MT; k++) { o[k][nt][e] *= c; o[k][nt][e + 2] *= c; }
@@ -353,10 +390,10 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
             uint32_t pf[2][NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                const float z0 = (m[nt][0] == -INFINITY ? 0.0f : m[nt][0]) - 10.0f, z1 = (m[nt][1] == -INFINITY ? 0.0f : m[nt][1]) - 10.0f;
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const float p0 = ex2(s[u][nt][0] - z0), p1 = ex2(s[u][nt][1] - z1), p2 = ex2(s[u][nt][2] - z0), p3 = ex2(s[u][nt][3] - z1);
+                    const float p0 = ex2(s[u][nt][0] - z[nt][0]), p1 = ex2(s[u][nt][1] - z[nt][1]);
+                    const float p2 = ex2(s[u][nt][2] - z[nt][0]), p3 = ex2(s[u][nt][3] - z[nt][1]);
                     l[nt][0] += p0 + p2;
                     l[nt][1] += p1 + p3;
                     pf[u][nt][0] = transpose8(pack_h2(p0, p1));
@@ -383,9 +420,9 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
                             if (__hisnan(e[c]) || __hisinf(e[c])) {
                                 f[c] = __ushort_as_half(0);
                                 const int k = key + ra + (c & 1) + 8 * (c >> 1);
-                                for (int col = 0; col < 8 * NT; col++) {
+                                for (int col = 0; col < 8 * NT && !((hole >> u) & 1); col++) {
                                     const int cc = c0 + col;
-                                    if (cc < n_cols && k < k1 && k < visible(rq, rq.row0 + cc / G, a.frame)) atomicOr(&s_poison[col], 1u << grp);
+                                    if (cc < n_cols && k < k1 && k < visible(rq, s_col[col].x, a.frame)) atomicOr(&s_poison[col], 1u << grp);
                                 }
                             }
                         }
@@ -395,9 +432,9 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
                     uint32_t w[4];
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
-                        const int pos = row_pos(ra + (c & 1) + 8 * (c >> 1));
-                        if (NG % 2) w[c] = *(const uint16_t *) (vb + pos * RB + 16 * j + 2 * g);
-                        else w[c] = *(const uint32_t *) (vb + pos * RB + 16 * chunk_pos<NG>(pos, 2 * j + (g >> 2)) + 4 * (g & 3));
+                        const uint8_t * p = vb + v_at[c & 1] + (16 * u + 8 * (c >> 1)) * RB;
+                        if (NG % 2) w[c] = *(const uint16_t *) (p + 16 * j);
+                        else w[c] = *(const uint32_t *) (j ? p + v_step[c & 1] : p);
                     }
 #pragma unroll
                     for (int h = 0; h < (NG % 2 ? 1 : 2); h++) {
@@ -431,7 +468,7 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
                 const int col = warp * 8 * NT + 8 * nt + 2 * t + e;
-                if (g == 0) sm[col] = make_float2(m[nt][e], x);
+                if (g == 0) sm[col] = make_float2(z[nt][e], x);
 #pragma unroll
                 for (int k = 0; k < MT; k++) {
                     const int c = NG % 2 ? 32 * (k / 2) + 4 * g + 2 * (k % 2) : 64 * (k / 4) + 8 * g + 2 * (k % 4);
@@ -443,22 +480,21 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
         for (int idx = threadIdx.x; idx < 8 * NT * (HD / 4); idx += 32 * WARPS) {
             const int col = idx / (HD / 4), c = idx % (HD / 4) * 4;
             if (c0 + col >= n_cols) continue;
-            float top = -INFINITY, sum = 0.0f;
+            float top = -FLT_MAX, sum = 0.0f;
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < WARPS; w++) top = fmaxf(top, sm[w * 8 * NT + col].x);
 #pragma unroll
             for (int w = 0; w < WARPS; w++) {
+                // (a warp that saw nothing has zeros, or what a score that is not a number has made of them: kept by 0 * NaN)
                 const float2 ml = sm[w * 8 * NT + col];
-                const float f = ml.x == -INFINITY ? 0.0f : ml.x == top ? 1.0f : ex2(ml.x - top);
+                const float f = ml.x == top ? 1.0f : ex2(ml.x - top);
                 const float4 x = *(const float4 *) (so + (w * 8 * NT + col) * (HD + 4) + c);
-                // a warp that saw nothing holds zeros, or what a score that is not a number has made of them
-                const float k = ml.x == -INFINITY ? 1.0f : f;
-                sum = __fmaf_rn(ml.y, k, sum);
-                v.x = __fmaf_rn(x.x, k, v.x); v.y = __fmaf_rn(x.y, k, v.y); v.z = __fmaf_rn(x.z, k, v.z); v.w = __fmaf_rn(x.w, k, v.w);
+                sum = __fmaf_rn(ml.y, f, sum);
+                v.x = __fmaf_rn(x.x, f, v.x); v.y = __fmaf_rn(x.y, f, v.y); v.z = __fmaf_rn(x.z, f, v.z); v.w = __fmaf_rn(x.w, f, v.w);
             }
             if ((s_poison[col] >> (c / 32)) & 1) v.x = v.y = v.z = v.w = __int_as_float(0x7fffffff);
-            const int row = rq.row0 + (c0 + col) / G, head = kh * G + (c0 + col) % G;
+            const int row = s_col[col].x, head = s_col[col].y;
             if (used <= 1) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 T * out = (T *) a.out + (long long) row * a.o_tok + head * a.o_head + c;
@@ -494,7 +530,7 @@ __global__ void __launch_bounds__(256) k_kv4_merge(const Kv4Pool pool, const Kv4
     if (used <= 1) return;                                   // written by the first kernel
     for (int row = rq.row0 + blockIdx.x; row < rq.row1; row += gridDim.x) {
         const size_t at = (size_t) row * a.heads + head, step = (size_t) a.n_rows * a.heads;
-        float top = -INFINITY;
+        float top = -FLT_MAX;
         for (int s = threadIdx.x; s < used; s += 256) top = fmaxf(top, sp.ml[at + s * step].x);
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
@@ -508,7 +544,7 @@ __global__ void __launch_bounds__(256) k_kv4_merge(const Kv4Pool pool, const Kv4
 #pragma unroll 4
         for (int s = warp; s < used; s += 8) {
             const float2 ml = sp.ml[at + s * step];
-            const float f = ml.x == top || ml.x == -INFINITY ? 1.0f : ex2(ml.x - top);   // -inf: zeros, or NaN to be kept
+            const float f = ml.x == top ? 1.0f : ex2(ml.x - top);
             sum = __fmaf_rn(ml.y, f, sum);
 #pragma unroll
             for (int i = 0; i < NG; i++) v[i] = __fmaf_rn(sp.o[(at + s * step) * HD + 32 * i + lane], f, v[i]);
@@ -537,10 +573,13 @@ RowsPlan rows_plan(const Kv4Pool & p, const Kv4Attn & a) {
     const long long cols = (long long) a.max_new * (a.heads / p.heads);
     r.nt = cols > 8 ? 2 : 1;
     r.tiles = (int) std::min<long long>((cols + 8 * r.nt - 1) / (8 * r.nt), 65535 / p.heads);
-    // about 148 SMs x 4 CTAs x 3 ranges of equal length if every request is as long as the longest; 256 keys at least
-    const long long total = (long long) a.n_req * p.heads * r.tiles * a.max_len;
-    const long long chunk = std::max<long long>(256, (total / (148 * 4 * 3) + 127) & ~127LL);
-    r.sp.chunk = (int) std::min<long long>(chunk, 0x7fffff00);
+    // Ranges of 1024 keys or more, 4 to each of the 148 SMs x 4 resident CTAs if every request is as long as the longest
+    // (fewer leave SMs idle at the end where lengths differ, more pay for starts and partial sums; 64 sessions of
+    // 1000 .. 8190 keys: 768 / 1536 / 2048 / 4096 keys a range = 121 / 115 / 116 / 126 us); down to 256 keys when a range
+    // for each CTA is shorter than that.
+    const long long total = (long long) a.n_req * p.heads * r.tiles * a.max_len, slots = 148 * 4;
+    const long long chunk = std::max(std::max(256LL, std::min(1024LL, total / slots)), total / (4 * slots));
+    r.sp.chunk = (int) std::min<long long>((chunk + 127) & ~127LL, 0x7fffff00);
     r.sp.n_split = (a.max_len + r.sp.chunk - 1) / r.sp.chunk;
     r.sp.o = nullptr;
     r.sp.ml = nullptr;
