@@ -20,12 +20,10 @@
 // (the four states are merged at the end); the maximum is raised, and the sums rescaled, only when a score passes it
 // by 2^4, so most steps do no reduction across lanes. A long context is split over CTAs, whose partial sums
 // k_kv4_merge joins.
-#include "kv4.h"
+#include "kv4_device.h"
 #include "common.h"
 #include "launch.h"
 #include "kprof.h"
-
-#include <cuda_bf16.h>
 
 #include <algorithm>
 #include <cfloat>
@@ -34,52 +32,6 @@
 namespace jb {
 
 namespace {
-
-template <class T> __device__ __forceinline__ T to_type(float x);
-template <> __device__ __forceinline__ __half to_type(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ __nv_bfloat16 to_type(float x) { return __float2bfloat16_rn(x); }
-__device__ __forceinline__ float from_type(__half x) { return __half2float(x); }
-__device__ __forceinline__ float from_type(__nv_bfloat16 x) { return __bfloat162float(x); }
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// how a request's keys are divided: n_split ranges of `chunk` keys, longer ones where that does not cover them
-struct Split {
-    int n_split, chunk;
-    float * o;                  // [n_split][n_rows][heads][hd] partial sums
-    float2 * ml;                // [n_split][n_rows][heads] (maximum, sum)
-    __host__ __device__ int span(int len) const {
-        const int even = (len + n_split - 1) / n_split;
-        return even <= chunk ? chunk : (even + 127) & ~127;
-    }
-    __host__ __device__ int used(int len) const { return len > 0 ? (len + span(len) - 1) / span(len) : 0; }
-};
-
-// What a CTA needs to know of its request: rows [row0, row1) of q, keys [0, len) of the table.
-struct Req {
-    int row0, row1, last, len, lens;
-};
-__device__ __forceinline__ Req request_of(const Kv4Attn & a, int page_shift, int r) {
-    Req q;
-    q.last = a.q_start[r + 1];
-    q.row0 = max(0, a.q_start[r]);
-    q.row1 = min(q.last, a.n_rows);
-    q.lens = a.lens[r];
-    q.len = (int) min((long long) max(q.lens, 0), (long long) a.width << page_shift);
-    return q;
-}
-// keys that row `row` sees
-__device__ __forceinline__ int visible(const Req & q, int row, int frame) {
-    if (frame == 0) return q.len;
-    const int p = q.lens - q.last + row;
-    if (p < 0) return 0;
-    const long long lim = ((long long) p / frame + 1) * frame;
-    return lim < q.len ? (int) lim : q.len;
-}
 
 __device__ __forceinline__ uint32_t smem_addr(const void * p) { return (uint32_t) __cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void * src) {
@@ -106,29 +58,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *(const uint32_t *) &h;
-}
-__device__ __forceinline__ uint32_t h2u(__half2 h) { return *(const uint32_t *) &h; }
-__device__ __forceinline__ __half2 u2h(uint32_t u) { return *(const __half2 *) &u; }
-
-// The nibbles 0 .. 3 of both 16-bit halves of u as four half2 of the integers -8 .. 7: 0x6400 | c is 1024 + c in f16,
-// 0x6400 | 16 c is 1024 + 16 c; both steps are exact.
-__device__ __forceinline__ uint32_t and_or(uint32_t u, uint32_t mask) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(u), "r"(mask), "r"(0x64006400u));
-    return r;
-}
-__device__ __forceinline__ void codes4(uint32_t u, __half2 (&x)[4]) {
-    const __half2 bias = u2h(0xe408e408u), sixteenth = u2h(0x2c002c00u), bias16 = u2h(0xd480d480u);   // -1032, 1/16, -72
-    const uint32_t v = u >> 8;
-    x[0] = __hadd2(u2h(and_or(u, 0x000f000fu)), bias);
-    x[1] = __hfma2(u2h(and_or(u, 0x00f000f0u)), sixteenth, bias16);
-    x[2] = __hadd2(u2h(and_or(v, 0x000f000fu)), bias);
-    x[3] = __hfma2(u2h(and_or(v, 0x00f000f0u)), sixteenth, bias16);
-}
-
 constexpr int STEP = 32;        // keys a warp takes at a time
 constexpr int STAGES = 3;
 constexpr int WARPS = 4;
@@ -366,7 +295,7 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     mx[nt][e] = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
-                    raise = raise || mx[nt][e] > z[nt][e] + 14.0f;
+                    raise = raise || mx[nt][e] - z[nt][e] > 14.0f;
                 }
             }
             if (__any_sync(0xffffffffu, raise)) {
@@ -377,7 +306,7 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
                         float x = mx[nt][e];
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                        x = fmaxf(x - 10.0f, z[nt][e]);
+                        x = fmaxf(below(x), z[nt][e]);
                         const float c = x == z[nt][e] ? 1.0f : ex2(z[nt][e] - x);
                         z[nt][e] = x;
                         l[nt][e] *= c;
@@ -563,21 +492,24 @@ __global__ void __launch_bounds__(256) k_kv4_merge(const Kv4Pool pool, const Kv4
     }
 }
 
-// The launch of the rows kernel: columns a CTA takes, CTAs along the columns, and the division of the keys.
-struct RowsPlan {
+// The launch: which kernel, columns a CTA takes, CTAs along the columns, and the division of the keys.
+struct Plan {
+    bool tc;                    // the tiles kernel
     int nt, tiles;
     Split sp;
 };
-RowsPlan rows_plan(const Kv4Pool & p, const Kv4Attn & a) {
-    RowsPlan r;
+Plan plan_of(const Kv4Pool & p, const Kv4Attn & a) {
+    Plan r;
     const long long cols = (long long) a.max_new * (a.heads / p.heads);
+    r.tc = cols > 16;
     r.nt = cols > 8 ? 2 : 1;
-    r.tiles = (int) std::min<long long>((cols + 8 * r.nt - 1) / (8 * r.nt), 65535 / p.heads);
+    const int wide = r.tc ? 256 : 8 * r.nt;
+    r.tiles = (int) std::min<long long>((cols + wide - 1) / wide, 65535 / p.heads);
     // Ranges of 1024 keys or more, 4 to each of the 148 SMs x 4 resident CTAs if every request is as long as the longest
     // (fewer leave SMs idle at the end where lengths differ, more pay for starts and partial sums; 64 sessions of
     // 1000 .. 8190 keys: 768 / 1536 / 2048 / 4096 keys a range = 121 / 115 / 116 / 126 us); down to 256 keys when a range
     // for each CTA is shorter than that.
-    const long long total = (long long) a.n_req * p.heads * r.tiles * a.max_len, slots = 148 * 4;
+    const long long total = (long long) a.n_req * p.heads * r.tiles * a.max_len, slots = r.tc ? 148 : 148 * 4;
     const long long chunk = std::max(std::max(256LL, std::min(1024LL, total / slots)), total / (4 * slots));
     r.sp.chunk = (int) std::min<long long>((chunk + 127) & ~127LL, 0x7fffff00);
     r.sp.n_split = (a.max_len + r.sp.chunk - 1) / r.sp.chunk;
@@ -591,7 +523,7 @@ size_t partial_bytes(const Kv4Pool & p, const Kv4Attn & a, int n_split) {
 }
 
 template <class T, int NG, int NT>
-int rows_launch(const Kv4Pool & p, const Kv4Attn & a, RowsPlan r, int vec, cudaStream_t st) {
+int rows_launch(const Kv4Pool & p, const Kv4Attn & a, const Plan & r, int vec, cudaStream_t st) {
     constexpr int smem = rows_smem<NG, NT>();
     JB_CUDA(cudaFuncSetAttribute(k_kv4_rows<T, NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     const dim3 grid((unsigned) r.sp.n_split, (unsigned) (p.heads * r.tiles), (unsigned) a.n_req);
@@ -601,15 +533,17 @@ int rows_launch(const Kv4Pool & p, const Kv4Attn & a, RowsPlan r, int vec, cudaS
 
 template <class T, int NG>
 int launch(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st) {
-    RowsPlan r = rows_plan(p, a);
+    Plan r = plan_of(p, a);
     if (r.sp.n_split > 1) {
         r.sp.o = (float *) a.ws;
         r.sp.ml = (float2 *) (r.sp.o + (size_t) r.sp.n_split * a.n_rows * a.heads * p.hd);
     }
-    // 16-byte loads of q, 8-byte stores of out where the strides allow them
+    // 16-byte loads of q, 8- and 16-byte stores of out where the strides allow them
     const int vec = (((uintptr_t) a.q & 15) == 0 && ((a.q_tok | a.q_head) & 7) == 0 ? 1 : 0) |
-                    (((uintptr_t) a.out & 7) == 0 && ((a.o_tok | a.o_head) & 3) == 0 ? 2 : 0);
-    if (r.nt == 1 ? rows_launch<T, NG, 1>(p, a, r, vec, st) : rows_launch<T, NG, 2>(p, a, r, vec, st)) return -1;
+                    (((uintptr_t) a.out & 7) == 0 && ((a.o_tok | a.o_head) & 3) == 0 ? 2 : 0) |
+                    (((uintptr_t) a.out & 15) == 0 && ((a.o_tok | a.o_head) & 7) == 0 ? 4 : 0);
+    if (r.tc ? kv4_tiles(p, a, r.sp, r.tiles, vec, st)
+             : r.nt == 1 ? rows_launch<T, NG, 1>(p, a, r, vec, st) : rows_launch<T, NG, 2>(p, a, r, vec, st)) return -1;
     if (r.sp.n_split > 1) {
         const dim3 grid((unsigned) std::max(1, a.max_new), (unsigned) a.heads, (unsigned) a.n_req);
         JB_CUDA(launch_pdl(k_kv4_merge<T, NG>, grid, dim3(256), 0, st, p, a, r.sp));
@@ -631,7 +565,7 @@ int launch_dim(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st) {
 
 size_t kv4_attention_workspace(const Kv4Pool & p, const Kv4Attn & a) {
     if (!a.n_req || !a.n_rows) return 0;
-    return partial_bytes(p, a, rows_plan(p, a).sp.n_split);
+    return partial_bytes(p, a, plan_of(p, a).sp.n_split);
 }
 
 int kv4_attention(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st) {
