@@ -33,6 +33,10 @@ namespace jb {
 
 namespace {
 
+// The subtrahend z of a score s in its weight 2^(s - z), for a largest score m: m - 10, so that weights go up to 2^10 (2^14
+// before z is raised), within f16; m itself where m - 10 would be rounded (|m| > 2^20), so that s - z <= 0 there.
+__device__ __forceinline__ float below(float m) { return fabsf(m) > 0x1p20f ? m : m - 10.0f; }
+
 __device__ __forceinline__ uint32_t smem_addr(const void * p) { return (uint32_t) __cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void * src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(dst), "l"(src) : "memory");

@@ -20,10 +20,6 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// The subtrahend z of a score s in its weight 2^(s - z), for a largest score m: m - 10, so that weights go up to 2^10 (2^14
-// before z is raised), within f16; m itself where m - 10 would be rounded (|m| > 2^20), so that s - z <= 0 there.
-__device__ __forceinline__ float below(float m) { return fabsf(m) > 0x1p20f ? m : m - 10.0f; }
-
 // how a request's keys are divided: n_split ranges of `chunk` keys, longer ones where that does not cover them
 struct Split {
     int n_split, chunk;

@@ -41,15 +41,16 @@ def ref_attention(q, k, v, pos, frame, scale):
     z = p.sum(1, keepdim=True)
     p = p / torch.where(z == 0, 1.0, z)
     size = (q.abs() @ k.abs().T * abs(scale)).masked_fill(~see, 0.0)
-    # the mean of |v|, with the weights' step at the small end of f16 added (see bound): 2^-35 of |v| for every key seen
-    mean = p @ v.abs() + 2.0 ** -24 * (see.double() @ v.abs())
+    # the mean of |v|, with the weights' step at the small end of f16 added (see bound): 2^-31 of |v| for every key seen
+    mean = p @ v.abs() + 2.0 ** -20 * (see.double() @ v.abs())
     return p @ v, mean, size.amax(1, keepdim=True) if L else torch.zeros(q.shape[0], 1, dtype=torch.float64)
 
 
 def bound(ref, mean_abs, size, dtype):
     # the output's rounding, half a step of its type; the weights' rounding to f16, half a step of each: 2^-11 of a
-    # normal one, 2^-25 of a subnormal one, where the weights are scaled so that the largest is at least 2^10 -- so
-    # at most 2^-11 w + 2^-35 w_max, and w_max / sum(w) <= 1: mean_abs carries the second part as 2^-11 * 2^-24;
+    # normal one, 2^-25 of a subnormal one, where the weights are scaled so that the largest is at least 2^6 (many rows;
+    # 2^10 few rows) -- so at most 2^-11 w + 2^-31 w_max, and w_max / sum(w) <= 1: mean_abs carries the second part
+    # as 2^-11 * 2^-20;
     # the scores' f32 sums of up to 128 products and the exponent's product: |error| <= 2^-18 of the sum of magnitudes,
     # which moves a weight by that much of itself, numerator and denominator both
     half = torch.finfo(dtype).eps / 2
