@@ -81,7 +81,7 @@ template <int NG> __device__ __forceinline__ int chunk_pos(int pos, int c) { ret
 
 template <class T, int NG, int NT>
 __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const Kv4Pool pool, const Kv4Attn a, const Split sp, int tiles,
-                                                                          int vec) {
+                                                                          int vec, int rest) {
     constexpr int HD = 32 * NG, RB = row_bytes<NG>(), SB = stage_bytes<NG>(), MT = 2 * NG;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -114,7 +114,8 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
     // .. and from there to the second 64 channels (of four-chunk rows: the other two chunks, which side depends on the row)
     const int v_step[2] = {NG == 4 && (v_a & 2) ? -32 : 32, NG == 4 && (v_b & 2) ? -32 : 32};
 
-    for (int c0 = (int) (blockIdx.y % tiles) * 8 * NT; c0 < n_cols; c0 += tiles * 8 * NT) {
+    // rest: only the columns that the tiles kernel leaves
+    for (int c0 = (rest ? tile_columns(n_cols) : 0) + (int) (blockIdx.y % tiles) * 8 * NT; c0 < n_cols; c0 += tiles * 8 * NT) {
         if (threadIdx.x < 8 * NT) s_poison[threadIdx.x] = 0;
         // ---- the tile's columns: lane (g, t) loads channels 32 i + 8 t .. + 7 of column g of each 8
         uint32_t qf[NT][NG][4];
@@ -506,9 +507,9 @@ Plan plan_of(const Kv4Pool & p, const Kv4Attn & a) {
     Plan r;
     const long long cols = (long long) a.max_new * (a.heads / p.heads);
     r.tc = cols > 16;
-    r.nt = cols > 8 ? 2 : 1;
-    const int wide = r.tc ? 256 : 8 * r.nt;
-    r.tiles = (int) std::min<long long>((cols + wide - 1) / wide, 65535 / p.heads);
+    r.nt = (r.tc ? cols % 256 : cols) > 8 ? 2 : 1;
+    if (r.tc) r.tiles = (int) std::min<long long>((cols + 255 - 16) / 256, 65535 / p.heads);
+    else r.tiles = (int) std::min<long long>((cols + 8 * r.nt - 1) / (8 * r.nt), 65535 / p.heads);
     // Ranges of 1024 keys or more, 4 to each of the 148 SMs x 4 resident CTAs if every request is as long as the longest
     // (fewer leave SMs idle at the end where lengths differ, more pay for starts and partial sums; 64 sessions of
     // 1000 .. 8190 keys: 768 / 1536 / 2048 / 4096 keys a range = 121 / 115 / 116 / 126 us); down to 256 keys when a range
@@ -528,10 +529,11 @@ size_t partial_bytes(const Kv4Pool & p, const Kv4Attn & a, int n_split) {
 
 template <class T, int NG, int NT>
 int rows_launch(const Kv4Pool & p, const Kv4Attn & a, const Plan & r, int vec, cudaStream_t st) {
+    const int tiles = r.tc ? 1 : r.tiles;
     constexpr int smem = rows_smem<NG, NT>();
     JB_CUDA(cudaFuncSetAttribute(k_kv4_rows<T, NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    const dim3 grid((unsigned) r.sp.n_split, (unsigned) (p.heads * r.tiles), (unsigned) a.n_req);
-    JB_CUDA(launch_pdl(k_kv4_rows<T, NG, NT>, grid, dim3(32 * WARPS), smem, st, p, a, r.sp, r.tiles, vec));
+    const dim3 grid((unsigned) r.sp.n_split, (unsigned) (p.heads * tiles), (unsigned) a.n_req);
+    JB_CUDA(launch_pdl(k_kv4_rows<T, NG, NT>, grid, dim3(32 * WARPS), smem, st, p, a, r.sp, tiles, vec, r.tc ? 1 : 0));
     return 0;
 }
 
@@ -546,8 +548,8 @@ int launch(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st) {
     const int vec = (((uintptr_t) a.q & 15) == 0 && ((a.q_tok | a.q_head) & 7) == 0 ? 1 : 0) |
                     (((uintptr_t) a.out & 7) == 0 && ((a.o_tok | a.o_head) & 3) == 0 ? 2 : 0) |
                     (((uintptr_t) a.out & 15) == 0 && ((a.o_tok | a.o_head) & 7) == 0 ? 4 : 0);
-    if (r.tc ? kv4_tiles(p, a, r.sp, r.tiles, vec, st)
-             : r.nt == 1 ? rows_launch<T, NG, 1>(p, a, r, vec, st) : rows_launch<T, NG, 2>(p, a, r, vec, st)) return -1;
+    if (r.tc && kv4_tiles(p, a, r.sp, r.tiles, vec, st)) return -1;
+    if (r.nt == 1 ? rows_launch<T, NG, 1>(p, a, r, vec, st) : rows_launch<T, NG, 2>(p, a, r, vec, st)) return -1;
     if (r.sp.n_split > 1) {
         const dim3 grid((unsigned) std::max(1, a.max_new), (unsigned) a.heads, (unsigned) a.n_req);
         JB_CUDA(launch_pdl(k_kv4_merge<T, NG>, grid, dim3(256), 0, st, p, a, r.sp));

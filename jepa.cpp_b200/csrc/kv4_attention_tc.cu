@@ -2,8 +2,8 @@
 //
 // One CTA per (request, cache head, 256 columns, range of keys); a column is a (new token, head of the group) pair, a
 // row of the two 128-row tiles here. Keys come in blocks of 64. Warps:
-//   0 .. 7   softmax: one thread per row (4 warps a tile, one per TMEM lane quadrant). They write the queries into shared
-//            memory once (scaled by a power of two into f16's range), then per block read their row of S = Q K^T from
+//   0 .. 7   softmax: one thread per row (4 warps a tile, one per TMEM lane quadrant). They write the queries into TMEM
+//            once (scaled by a power of two into f16's range), then per block read their row of S = Q K^T from
 //            TMEM once, and put the weights P = 2^(s - z) back in f16 over the front half of S's
 //            columns, where the second product takes it as its A operand: P never passes through shared memory.
 //            O stays in TMEM; it is rescaled only when a weight would pass 2^14.5 (they start from 2^6 .. 2^7 at the
@@ -11,12 +11,13 @@
 //   8 .. 11  conversion from 4 bits to d (c - 8) in f16 (exact, kv4.h), one thread per row: two warps for K, two for V,
 //            written in the 128-byte swizzle of the products' operands (K: K-major; V: MN-major, keys down
 //            the rows). The next block's codes are loaded before this one's are converted; four blocks are held.
-//   12, 13   issue the products of tile 0 and 1: S_t = Q_t K^T (M 128, N 64), two blocks ahead in two buffers, and
-//            O_t += P_t V (M 128, N hd). Softmax never waits for a product of its own block, and the tiles run on
-//            their own. (128 keys at once with one buffer of S: 2200 cycles a block were spent waiting for it.)
+//   12, 13   issue the products of tile 0 and 1: S_t = Q_t K^T (M 128, N 64) and O_t += P_t V (M 128, N hd). Both take A from
+//            TMEM: the tensor core reads shared memory at about 64 bytes a cycle, so that with Q there too a 128 x 64 x 16
+//            product took 100 cycles instead of 32. Up to head_dim 64 TMEM has room for two buffers of S a tile, and
+//            the scores run two blocks ahead; above that the tiles' turns hide each other's products.
 // Within 8 channels the operands keep the order in which codes unpack, 0 4 1 5 2 6 3 7: Q is written in the order of
 // K's words, O's columns are put right when they are stored.
-// TMEM: S of tile t, buffer b at column 128 t + 64 b, O of tile t at 256 + 128 t.
+// TMEM columns: O_0, O_1 (hd each), Q_0, Q_1 (hd / 2), then the buffers of S.
 // A value scale that is not finite enters as zeros; the rows that see such a key get NaN in that group at the end, so a NaN
 // behind a row's mask does not reach it (0 * NaN).
 // Every mbarrier wait is bounded: on a timeout the kernel raises the error flag, its rows become NaN, and it ends.
@@ -87,6 +88,9 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -125,16 +129,20 @@ __device__ __forceinline__ bool warp_wait(uint64_t * bar, uint32_t parity, int c
 __device__ __forceinline__ uint32_t seen(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
 template <int NG> __host__ __device__ constexpr int atoms() { return (NG + 1) / 2; }
-template <int NG> constexpr size_t tiles_smem() { return (size_t) atoms<NG>() * (2 * QATOM + 2 * STAGES * ATOM) + 1024; }
+template <int NG> constexpr size_t tiles_smem() { return (size_t) atoms<NG>() * ((NG <= 2 ? 0 : 2 * QATOM) + 2 * STAGES * ATOM) + 1024; }
 
 template <class T, int NG>
 __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, const Kv4Attn a, const Split sp, int tiles, int vec) {
     constexpr int HD = 32 * NG, AT = atoms<NG>(), W = 4 * NG;      // W: 8-channel words of a row
+    constexpr bool QT = NG <= 2;                                   // Q in tensor memory, else in shared memory
+    constexpr int NB = 2;                                          // buffers of S a tile
+    constexpr uint32_t Q_COL = 2 * HD, S_COL = QT ? 3 * HD : 2 * HD;
+    static_assert(S_COL + 2 * NB * BLK <= 512, "tensor memory");
     extern __shared__ uint8_t smem_raw[];
-    uint8_t * sQ = (uint8_t *) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
-    uint8_t * sK = sQ + 2 * AT * QATOM, * sV = sK + STAGES * AT * ATOM;
+    // shared addresses
+    const uint32_t sQ = (smem_u32(smem_raw) + 1023) & ~1023u, sK = sQ + (QT ? 0 : 2 * AT * QATOM), sV = sK + STAGES * AT * ATOM;
     struct Bars {
-        uint64_t k_full[STAGES], v_full[STAGES], k_empty[2][STAGES], v_empty[2][STAGES], s_full[2][2], p_full[2][2], o_done[2][2];   // [tile][stage or buffer]
+        uint64_t k_full[STAGES], v_full[STAGES], k_empty[2][STAGES], v_empty[2][STAGES], s_full[2][NB], p_full[2][NB], o_done[2][NB];   // [tile][stage or buffer]
     };
     __shared__ __align__(8) Bars bars;
     // per block and 32 keys: any exception; keys without a page; keys whose value scale of a group is not finite
@@ -147,7 +155,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
     const int warp = __shfl_sync(0xffffffffu, (int) (threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // warp: uniform to the compiler
     const int kh = blockIdx.y / tiles, r = blockIdx.z, G = a.heads / pool.heads;
     const Req rq = request_of(a, pool.page_shift, r);
-    const int n_cols = (rq.row1 - rq.row0) * G;
+    const int n_cols = tile_columns((rq.row1 - rq.row0) * G);
     const int span = sp.span(rq.len), used = sp.used(rq.len);
     const int k0 = blockIdx.x * span;
     if (n_cols <= 0 || (int) (blockIdx.y % tiles) * 256 >= n_cols || (blockIdx.x && (int) blockIdx.x >= used)) return;
@@ -164,6 +172,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
         const int nb_all = kend > k0 ? (kend - k0 + BLK - 1) / BLK : 0;
         const int kend0 = n_tiles == 1 ? kend : min(visible(rq, rq.row0 + (c0 + 127) / G, a.frame), kend);
         const int nb0 = kend0 > k0 ? (kend0 - k0 + BLK - 1) / BLK : 0;          // blocks of tile 0
+        fence_before();
+        __syncthreads();                        // TMEM is there, and free of the columns before
+        fence_after();
+        const uint32_t tmem = tmem_sh;
         if (threadIdx.x == 0) {
             for (int s = 0; s < STAGES; s++) {
                 mbar_init(&bars.k_full[s], CONV / 2);
@@ -171,8 +183,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                 for (int t = 0; t < 2; t++) { mbar_init(&bars.k_empty[t][s], 1); mbar_init(&bars.v_empty[t][s], 1); }
             }
             for (int t = 0; t < 2; t++) {
-                // (of blocks in turn: a warp may be a block ahead of another, and two products ahead of the last that is done)
-                for (int i = 0; i < 2; i++) {
+                // (one a buffer: a warp may be as many blocks ahead of another)
+                for (int i = 0; i < NB; i++) {
                     mbar_init(&bars.s_full[t][i], 1);
                     mbar_init(&bars.o_done[t][i], 1);
                     mbar_init(&bars.p_full[t][i], (uint32_t) max(1, (min(128, cols - 128 * t) + 31) / 32));
@@ -217,21 +229,26 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
             // (not 0, which would make NaN of a masked score's -inf)
             f = fmaxf(fabsf(a.scale) * 1.4426950408889634f * __int_as_float((127 - ex) << 23), 1e-37f);
             if (there) lim = min(visible(rq, row, a.frame), kend);
-            uint8_t * dst = sQ + (warp >> 2) * AT * QATOM + (threadIdx.x & 127) * 128;
+            const uint32_t qc = tmem + ((uint32_t) (32 * (warp & 3)) << 16) + Q_COL + (warp >> 2) * (HD / 2);
+            const uint32_t qs = sQ + (warp >> 2) * AT * QATOM + (threadIdx.x & 127) * 128;
 #pragma unroll
-            for (int s = 0; s < W; s++) {
-                word(s, x);
-                uint4 w;
-                w.x = pack_h2(x[0] * up, x[4] * up); w.y = pack_h2(x[1] * up, x[5] * up);
-                w.z = pack_h2(x[2] * up, x[6] * up); w.w = pack_h2(x[3] * up, x[7] * up);
-                *(uint4 *) (dst + (s / 8) * QATOM + (((s & 7) ^ (lane & 7)) << 4)) = w;
+            for (int s = 0; s < W; s += 4) {
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    word(s + i, x);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) w[4 * i + c] = pack_h2(x[c] * up, x[c + 4] * up);
+                    if (!QT) st_shared16(qs + ((s + i) / 8) * QATOM + ((((s + i) & 7) ^ (lane & 7)) << 4), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                }
+                if (QT) tmem_st16(qc + 4 * s, w);
             }
-            fence_async();
+            tmem_wait_st();
+            fence_async();                      // (the barriers)
         }
         fence_before();
         __syncthreads();
         fence_after();
-        const uint32_t tmem = tmem_sh;
 
         if (warp >= SOFT && warp < SOFT + CONV) {
             // ---- conversion: thread = a K row (warps 8, 9) or a V row (10, 11) of the block
@@ -239,7 +256,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
             const bool keys = warp < SOFT + 2;
             const int32_t * table = a.table + (size_t) r * a.width;
             const int n_pages = (int) (pool.n_slots >> pool.page_shift), pmask = (1 << pool.page_shift) - 1, P = 1 << pool.page_shift;
-            const uint32_t d_plane = ((uint32_t) pool.heads * NG) << pool.page_shift;      // scales from a key to its value
+            // this head's rows and scales of page 0, and from page to page
+            const uint32_t d_plane = ((uint32_t) pool.heads * NG) << pool.page_shift, q_page = ((uint32_t) pool.heads << pool.page_shift) * 32 * NG;
+            const uint8_t * q_head = pool.q + kv4_q_at(pool, 0, keys ? 0 : 1, kh, 0);
+            const __half * d_head = pool.d + kv4_d_at(pool, 0, keys ? 0 : 1, kh, 0);
             auto page_at = [&](int key) -> int {
                 const int p = key < kend ? __ldg(table + (key >> pool.page_shift)) : -1;
                 return p < n_pages ? p : -1;
@@ -251,8 +271,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                 const int key = k0 + j * BLK + kt;
                 heldn = page;
                 if (page >= 0) {
-                    const uint4 * q = (const uint4 *) (pool.q + kv4_q_at(pool, page, keys ? 0 : 1, kh, key & pmask));
-                    const __half * s = pool.d + kv4_d_at(pool, page, keys ? 0 : 1, kh, key & pmask);
+                    const uint4 * q = (const uint4 *) (q_head + (uint64_t) (uint32_t) page * q_page + (key & pmask) * 16 * NG);
+                    const __half * s = d_head + (uint64_t) (uint32_t) page * (2 * d_plane) + (key & pmask);
 #pragma unroll
                     for (int i = 0; i < NG; i++) next[i] = q[i];
 #pragma unroll
@@ -295,7 +315,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                         if (__hisnan(d[i]) || __hisinf(d[i])) d[i] = __ushort_as_half(0);
                     }
                 }
-                uint8_t * dst = (keys ? sK : sV) + s * AT * ATOM + kt * 128;
+                const uint32_t dst = (keys ? sK : sV) + s * AT * ATOM + kt * 128;
 #pragma unroll
                 for (int i = 0; i < W; i++) {
                     const uint4 & q4 = raw[i / 4];
@@ -303,9 +323,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                     const __half2 d2 = __half2half2(keys ? d[i % NG] : d[i / 4]);       // a key row's groups take turns
                     __half2 x[4];
                     codes4(w, x);
-                    uint4 o;
-                    o.x = h2u(__hmul2(x[0], d2)); o.y = h2u(__hmul2(x[1], d2)); o.z = h2u(__hmul2(x[2], d2)); o.w = h2u(__hmul2(x[3], d2));
-                    *(uint4 *) (dst + (i / 8) * ATOM + (((i & 7) ^ (kt & 7)) << 4)) = o;
+                    st_shared16(dst + (i / 8) * ATOM + (((i & 7) ^ (kt & 7)) << 4), h2u(__hmul2(x[0], d2)), h2u(__hmul2(x[1], d2)),
+                                h2u(__hmul2(x[2], d2)), h2u(__hmul2(x[3], d2)));
                 }
                 fence_async();
                 __syncwarp();
@@ -315,46 +334,48 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
         } else if (warp >= SOFT + CONV) {
             // ---- products of tile t: the whole warp waits, one lane issues
             const int t = warp - SOFT - CONV, nb = t == 0 ? nb0 : t < n_tiles ? nb_all : 0;
-            const uint32_t q_desc = (uint32_t) sw128_desc(smem_u32(sQ) + t * AT * QATOM), k_desc = (uint32_t) sw128_desc(smem_u32(sK));
-            const uint32_t v_desc = (uint32_t) mn_desc(smem_u32(sV)), k_hi = (uint32_t) (sw128_desc(0) >> 32);     // (the same for all)
+            const uint32_t q_desc = (uint32_t) sw128_desc(sQ + t * AT * QATOM), k_desc = (uint32_t) sw128_desc(sK), v_desc = (uint32_t) mn_desc(sV), hi = (uint32_t) (sw128_desc(0) >> 32);
+            const uint32_t od = tmem + HD * t, qd = tmem + Q_COL + HD / 2 * t, sd = tmem + S_COL + NB * BLK * t;
             auto scores_of = [&](int j) -> bool {
                 const int s = j % STAGES;
                 if (!warp_wait(&bars.k_full[s], (uint32_t) (j / STAGES) & 1u, 43)) return false;
                 fence_after();
-                const uint32_t id = idesc((min(BLK, kend - k0 - j * BLK) + 15) & ~15, false), ds = tmem + 128u * t + 64u * (j & 1);
+                const uint32_t id = idesc((min(BLK, kend - k0 - j * BLK) + 15) & ~15, false), ds = sd + BLK * (j % NB);
                 const uint32_t k_lo = k_desc + s * (AT * ATOM >> 4);
                 if (elect_one()) {
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; kk++) {
-                        mma_ss(ds, q_desc + ((kk / 4) * QATOM + (kk % 4) * 32 >> 4), k_hi, k_lo + ((kk / 4) * ATOM + (kk % 4) * 32 >> 4), k_hi, id, kk != 0);
+                        const uint32_t kl = k_lo + ((kk / 4) * ATOM + (kk % 4) * 32 >> 4);
+                        if (QT) mma_ts(ds, qd + 8 * kk, kl, hi, id, kk != 0);
+                        else mma_ss(ds, q_desc + ((kk / 4) * QATOM + (kk % 4) * 32 >> 4), hi, kl, hi, id, kk != 0);
                     }
-                    mma_commit(&bars.s_full[t][j & 1]);
+                    mma_commit(&bars.s_full[t][j % NB]);
                     mma_commit(&bars.k_empty[t][s]);
                 }
                 __syncwarp();
                 return true;
             };
             bool ok = true;
-            for (int j = 0; j < 2 && j < nb && ok; j++) ok = scores_of(j);
+            for (int j = 0; j < NB && j < nb && ok; j++) ok = scores_of(j);
             for (int j = 0; j < nb && ok; j++) {
                 const int s = j % STAGES;
-                ok = warp_wait(&bars.p_full[t][j & 1], (uint32_t) (j >> 1) & 1u, 44) && warp_wait(&bars.v_full[s], (uint32_t) (j / STAGES) & 1u, 45);
+                ok = warp_wait(&bars.p_full[t][j % NB], (uint32_t) (j / NB) & 1u, 44) && warp_wait(&bars.v_full[s], (uint32_t) (j / STAGES) & 1u, 45);
                 if (!ok) break;
                 fence_after();
                 const int steps = (min(BLK, kend - k0 - j * BLK) + 15) / 16;
-                const uint32_t v_lo = v_desc + s * (AT * ATOM >> 4), pa = tmem + 128u * t + 64u * (j & 1), od = tmem + 256u + 128u * t;
+                const uint32_t v_lo = v_desc + s * (AT * ATOM >> 4), pa = sd + BLK * (j % NB);
                 if (elect_one()) {
-                    mma_ts(od, pa, v_lo, k_hi, idesc(HD, true), j != 0);
+                    mma_ts(od, pa, v_lo, hi, idesc(HD, true), j != 0);
 #pragma unroll
                     for (int kk = 1; kk < BLK / 16; kk++) {
-                        if (kk < steps) mma_ts(od, pa + 8u * kk, v_lo + (kk * 2048 >> 4), k_hi, idesc(HD, true), 1);
+                        if (kk < steps) mma_ts(od, pa + 8u * kk, v_lo + (kk * 2048 >> 4), hi, idesc(HD, true), 1);
                     }
-                    mma_commit(&bars.o_done[t][j & 1]);
+                    mma_commit(&bars.o_done[t][j % NB]);
                     mma_commit(&bars.v_empty[t][s]);
                 }
                 __syncwarp();
-                // the scores two blocks on go over P_t(j): only when its product is done
-                if (j + 2 < nb) ok = warp_wait(&bars.o_done[t][j & 1], (uint32_t) (j >> 1) & 1u, 46) && scores_of(j + 2);
+                // the buffer's next scores go over P_t(j): only when its product is done
+                if (j + NB < nb) ok = warp_wait(&bars.o_done[t][j % NB], (uint32_t) (j / NB) & 1u, 46) && scores_of(j + NB);
             }
             // the last arrivals of the commits, so that none meets a barrier that is set up anew
             for (int s = 0; s < STAGES && ok; s++) {
@@ -366,12 +387,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
             // ---- softmax: thread = row
             const int t = warp >> 2, nb = t == 0 ? nb0 : nb_all;
             const uint32_t lanes = (uint32_t) (32 * (warp & 3)) << 16;
-            const uint32_t ts = tmem + lanes + 128u * t, to = tmem + lanes + 256u + 128u * t;
+            const uint32_t ts = tmem + lanes + S_COL + NB * BLK * t, to = tmem + lanes + HD * t;
             float z = col < n_cols ? -FLT_MAX : 0.0f, l = 0.0f;     // about the running maximum less 6 (a whole number), the sum of weights 2^(s - z)
             uint32_t poison = 0;
             bool ok = true, plain = false;
-            // O_t += P_t V of block j is done (a warp that asks has seen S(j) or S(j + 1), so block j - 2's is)
-            auto product_done = [&](int j, int code) -> bool { return warp_wait(&bars.o_done[t][j & 1], (uint32_t) (j >> 1) & 1u, code); };
+            // O_t += P_t V of block j is done (a warp that asks has seen S(j) or S(j + 1), so block j - NB's is)
+            auto product_done = [&](int j, int code) -> bool { return warp_wait(&bars.o_done[t][j % NB], (uint32_t) (j / NB) & 1u, code); };
             // Raises z of the rows whose largest s - z of a block is `top` > 14.5 (z is a whole number, and so is the step:
             // sums and O take an exact power of two); returns the step.
             auto raise = [&](float top, int j) -> float {
@@ -396,8 +417,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
             };
             for (int j = 0; j < nb && ok; j++) {
                 const int key = k0 + j * BLK;
-                const uint32_t tb = ts + 64u * (j & 1);
-                if (!warp_wait(&bars.s_full[t][j & 1], (uint32_t) (j >> 1) & 1u, 47)) { ok = false; break; }
+                const uint32_t tb = ts + BLK * (j % NB);
+                if (!warp_wait(&bars.s_full[t][j % NB], (uint32_t) (j / NB) & 1u, 47)) { ok = false; break; }
                 fence_after();
                 uint32_t x[2][32];
                 tmem_ld32_async(tb, x[0]);
@@ -479,10 +500,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                 uint64_t sum2[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) x[h][i] = __float_as_uint(ex2(__uint_as_float(x[h][i])));
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const float p0 = ex2(__uint_as_float(x[h][2 * i])), p1 = ex2(__uint_as_float(x[h][2 * i + 1]));
+                        const float p0 = __uint_as_float(x[h][2 * i]), p1 = __uint_as_float(x[h][2 * i + 1]);
                         sum2[i & 3] = add2(sum2[i & 3], pack2(p0, p1));
                         p[i] = pack_h2(p0, p1);
                     }
@@ -493,7 +519,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                 tmem_wait_st();
                 fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.p_full[t][j & 1]);
+                if (lane == 0) mbar_arrive(&bars.p_full[t][j % NB]);
             }
             if (ok && nb > 0) ok = product_done(nb - 1, 49);
             if (!ok) abort_sh = 1;

@@ -54,6 +54,11 @@ __device__ __forceinline__ int visible(const Req & q, int row, int frame) {
     return lim < q.len ? (int) lim : q.len;
 }
 
+// Columns of a request and cache head that the tiles kernel takes, of n in all: whole tiles of 256, and what is left over if
+// it is more than 16; the rows kernel takes the rest. (258 columns in two CTAs of the tiles kernel: the second, for 2 of
+// them, took as long as the first.)
+__host__ __device__ inline int tile_columns(int n) { return n % 256 > 16 ? n : n - n % 256; }
+
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *(const uint32_t *) &h;
