@@ -531,7 +531,7 @@ template <class T, int NG, int NT>
 int rows_launch(const Kv4Pool & p, const Kv4Attn & a, const Plan & r, int vec, cudaStream_t st) {
     const int tiles = r.tc ? 1 : r.tiles;
     constexpr int smem = rows_smem<NG, NT>();
-    JB_CUDA(cudaFuncSetAttribute(k_kv4_rows<T, NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (allow_smem<k_kv4_rows<T, NG, NT>>(smem)) return -1;
     const dim3 grid((unsigned) r.sp.n_split, (unsigned) (p.heads * tiles), (unsigned) a.n_req);
     JB_CUDA(launch_pdl(k_kv4_rows<T, NG, NT>, grid, dim3(32 * WARPS), smem, st, p, a, r.sp, tiles, vec, r.tc ? 1 : 0));
     return 0;

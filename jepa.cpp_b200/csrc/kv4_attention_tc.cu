@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
 
 template <class T, int NG>
 int launch(const Kv4Pool & p, const Kv4Attn & a, const Split & sp, int tiles, int vec, cudaStream_t st) {
-    JB_CUDA(cudaFuncSetAttribute(k_kv4_tiles<T, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) tiles_smem<NG>()));
+    if (allow_smem<k_kv4_tiles<T, NG>>((int) tiles_smem<NG>())) return -1;
     const dim3 grid((unsigned) sp.n_split, (unsigned) (p.heads * tiles), (unsigned) a.n_req);
     JB_CUDA(launch_pdl(k_kv4_tiles<T, NG>, grid, dim3(THREADS), tiles_smem<NG>(), st, p, a, sp, tiles, vec));
     return 0;

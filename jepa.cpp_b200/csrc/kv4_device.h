@@ -3,8 +3,11 @@
 #pragma once
 
 #include "kv4.h"
+#include "common.h"
 
 #include <cuda_bf16.h>
+
+#include <atomic>
 
 namespace jb {
 
@@ -80,6 +83,19 @@ __device__ __forceinline__ void codes4(uint32_t u, __half2 (&x)[4]) {
     x[1] = __hfma2(u2h(and_or(u, 0x00f000f0u)), sixteenth, bias16);
     x[2] = __hadd2(u2h(and_or(v, 0x000f000fu)), bias);
     x[3] = __hfma2(u2h(and_or(v, 0x00f000f0u)), sixteenth, bias16);
+}
+
+// Lets kernel K have `bytes` of dynamic shared memory, once a device.
+template <auto K>
+int allow_smem(int bytes) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    JB_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = (uint64_t) 1 << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return 0;
+    JB_CUDA(cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+    return 0;
 }
 
 // The tiles kernel (kv4_attention_tc.cu): `grid` = (key ranges, cache heads x tiles of 256 columns, requests).

@@ -56,17 +56,21 @@ def _load() -> C.CDLL:
     return _lib
 
 
+def _stream(dev: torch.device) -> int:
+    """The raw handle of the device's current stream (without a torch.cuda.Stream object, which takes 3 us to make)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
 def _call(name: str, dev: torch.device, *args) -> None:
     """One call on the device's current stream (the C entry works on the current device)."""
-    L = _load()
-    fn = getattr(L, name)
+    fn = getattr(_lib or _load(), name)
     if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+        rc = fn(*args, _stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, _stream(dev))
     if rc != 0:
-        _raise(L, name)
+        _raise(_load(), name)
 
 
 def _raise(L: C.CDLL, name: str) -> None:
@@ -81,9 +85,10 @@ def _need(ok: bool, what: str) -> None:
 
 
 def _index(t: torch.Tensor, name: str, dtype: torch.dtype, dev: Optional[torch.device], dim: int = 1) -> None:
-    _need(isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == dim and t.is_contiguous(),
-          f"{name} must be a contiguous {dim}-D tensor of {dtype}")
-    _need(t.is_cuda and (dev is None or t.device == dev), f"{name} must be on the CUDA device of the others")
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == dim and t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous {dim}-D tensor of {dtype}")
+    if not (t.is_cuda and (dev is None or t.device == dev)):
+        raise ValueError(f"{name} must be on the CUDA device of the others")
 
 
 class Tables(NamedTuple):
@@ -110,7 +115,7 @@ def build_tables(cached: torch.Tensor, added: torch.Tensor, table: torch.Tensor,
     _need(1 <= n_slots < 2 ** 31, f"n_slots {n_slots} is not 1 .. 2^31 - 1")
     # lens, q_start and state share one allocation, each at a multiple of 4 bytes
     ints = torch.empty(2 * n + 3, dtype=torch.int32, device=dev)
-    lens, q_start, state = ints[:n], ints[n:2 * n + 1], ints[2 * n + 1:]
+    lens, q_start, state = ints.split((n, n + 1, 2))
     slots = torch.empty(n_slots, dtype=torch.int64, device=dev)
     base = ints.data_ptr()
     _call("jepa_b200_kv_tables", dev, cached.data_ptr(), added.data_ptr(), n, page_size, table.data_ptr(), table.shape[1],
@@ -151,23 +156,29 @@ class KV4Cache:
         self._ref = C.byref(self._c)
         self._dev = q.device
 
-    def _rows(self, t: torch.Tensor, name: str, heads: int) -> None:
-        _need(isinstance(t, torch.Tensor) and t.dim() == 3 and t.shape[1] == heads and t.shape[2] == self.head_dim,
-              f"{name} must be [rows, {heads}, {self.head_dim}]")
-        _need(t.device == self._dev, f"{name} must be on {self._dev}")
-        _need(t.stride(2) == 1, f"{name}'s channels must be contiguous")
+    def _rows(self, t: torch.Tensor, name: str, n: int, heads: int) -> Tuple[int, ...]:
+        """t is [n, heads, head_dim] on this device with contiguous channels; its strides."""
+        if not (isinstance(t, torch.Tensor) and t.shape == (n, heads, self.head_dim)):
+            raise ValueError(f"{name} must be [{n} rows, {heads}, {self.head_dim}]")
+        if t.device != self._dev:
+            raise ValueError(f"{name} must be on {self._dev}")
+        stride = t.stride()
+        if stride[2] != 1:
+            raise ValueError(f"{name}'s channels must be contiguous")
+        return stride
 
     def store(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Quantise rows k, v [n, kv_heads, head_dim] (f32, f16 or bf16, any strides of rows and heads) into slots [n]
         (int64; negative ones are skipped, the others must differ)."""
-        self._rows(k, "k", self.kv_heads)
-        self._rows(v, "v", self.kv_heads)
         _index(slots, "slots", torch.int64, self._dev)
-        _need(k.dtype in _TYPE and v.dtype is k.dtype, "k and v must be both f32, f16 or bf16")
         n = slots.shape[0]
-        _need(k.shape[0] == n and v.shape[0] == n, "k, v and slots must have one row a token")
-        _call("jepa_b200_kv4_store", self._dev, self._ref, k.data_ptr(), v.data_ptr(), _TYPE[k.dtype], k.stride(0), k.stride(1),
-              v.stride(0), v.stride(1), slots.data_ptr(), n)
+        ks = self._rows(k, "k", n, self.kv_heads)
+        vs = self._rows(v, "v", n, self.kv_heads)
+        kind = _TYPE.get(k.dtype)
+        if kind is None or v.dtype is not k.dtype:
+            raise ValueError("k and v must be both f32, f16 or bf16")
+        _call("jepa_b200_kv4_store", self._dev, self._ref, k.data_ptr(), v.data_ptr(), kind, ks[0], ks[1], vs[0], vs[1],
+              slots.data_ptr(), n)
 
     def load(self, slots: torch.Tensor, dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
         """The values cached in slots [n] (int64): k, v [n, kv_heads, head_dim]; zeros for a slot outside the pool."""
@@ -187,25 +198,27 @@ class KV4Cache:
         every cached key, 1 = causal, F = block-causal over frames of F tokens. max_len / max_new: bounds of lens and of
         a request's rows, which the launch is laid out for (they change no result). out (zeros by default) keeps the
         rows of no request."""
-        _need(q.dim() == 3, "q must be [rows, heads, head_dim]")
-        heads = q.shape[1]
-        self._rows(q, "q", heads)
-        _need(q.dtype is torch.float16 or q.dtype is torch.bfloat16, "q must be f16 or bf16")
+        _need(isinstance(q, torch.Tensor) and q.dim() == 3, "q must be [rows, heads, head_dim]")
+        rows, heads, _ = q.shape
+        qs = self._rows(q, "q", rows, heads)
+        if q.dtype is not torch.float16 and q.dtype is not torch.bfloat16:
+            raise ValueError("q must be f16 or bf16")
         _index(lens, "lens", torch.int32, self._dev)
         _index(q_start, "q_start", torch.int32, self._dev)
         _index(table, "table", torch.int32, self._dev, 2)
-        n = lens.shape[0]
-        _need(q_start.shape[0] == n + 1 and table.shape[0] == n, "lens, q_start and table must agree on the requests")
+        n, width = table.shape
+        if q_start.shape[0] != n + 1 or lens.shape[0] != n:
+            raise ValueError("lens, q_start and table must agree on the requests")
         if out is None:
-            out = torch.zeros(q.shape, dtype=q.dtype, device=self._dev)
-        else:
-            self._rows(out, "out", heads)
-            _need(out.dtype is q.dtype and out.shape[0] == q.shape[0], "out must be of q's type and shape")
-        a = _Attn(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), q_start.data_ptr(),
-                  lens.data_ptr(), table.data_ptr(), n, q.shape[0], table.shape[1], heads, _TYPE[q.dtype], frame,
+            out = torch.zeros((rows, heads, self.head_dim), dtype=q.dtype, device=self._dev)
+        elif out.dtype is not q.dtype:
+            raise ValueError("out must be of q's type")
+        os = self._rows(out, "out", rows, heads)
+        a = _Attn(q.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], q_start.data_ptr(), lens.data_ptr(),
+                  table.data_ptr(), n, rows, width, heads, _TYPE[q.dtype], frame,
                   1.0 / math.sqrt(self.head_dim) if scale is None else scale, max_len, max_new, None, 0)
         ref = C.byref(a)
-        L = _load()
+        L = _lib or _load()
         need = L.jepa_b200_kv4_attention_workspace(self._ref, ref)
         if need < 0:
             _raise(L, "jepa_b200_kv4_attention")

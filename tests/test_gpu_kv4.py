@@ -567,7 +567,7 @@ def test_refusals_on_the_device():
         c.attention(q, start, ln, table, frame=-1)
     with pytest.raises(RuntimeError, match="overlap"):
         c.attention(q, start, ln, table, out=torch.zeros(3, 1, 64, dtype=q.dtype, device="cuda").expand(3, 4, 64))
-    with pytest.raises(ValueError, match="one row a token"):
+    with pytest.raises(ValueError, match="k must be"):
         c.store(q[:, :2], q[:, :2], torch.arange(2, device="cuda"))
     with pytest.raises(ValueError, match="both f32"):
         c.store(q[:, :2], q[:, :2].float(), torch.arange(3, device="cuda"))
