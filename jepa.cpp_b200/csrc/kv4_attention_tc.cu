@@ -91,6 +91,11 @@ __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.
 __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -125,6 +130,8 @@ __device__ __forceinline__ bool warp_wait(uint64_t * bar, uint32_t parity, int c
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, code, &g_kv4_error));
 }
 
+// bits of an f16 infinity or NaN
+__device__ __forceinline__ bool not_finite(uint32_t h) { return (h & 0x7c00u) == 0x7c00u; }
 // the low n bits
 __device__ __forceinline__ uint32_t seen(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
@@ -192,26 +199,45 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
             }
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
-        // ---- queries: thread = row of the tiles, words in the order of the key rows
+        // ---- queries: first as they are into the stages' memory, by consecutive threads along the rows (a thread a row took
+        // 32 cache lines a load, 8,000 to 15,000 cycles in all), then thread = row of the tiles
+        constexpr int QB = 5;                   // words a thread has on their way at a time
+        for (int i0 = threadIdx.x; i0 < 256 * W; i0 += QB * THREADS) {
+            uint4 v[QB];
+#pragma unroll
+            for (int u = 0; u < QB; u++) {
+                const int i = i0 + u * THREADS, cc = c0 + i / W;
+                v[u] = make_uint4(0, 0, 0, 0);
+                if (i < 256 * W && cc < n_cols) {
+                    const T * q = (const T *) a.q + (long long) (rq.row0 + cc / G) * a.q_tok + (kh * G + cc % G) * a.q_head + 8 * (i % W);
+                    if (vec & 1) {
+                        v[u] = *(const uint4 *) q;
+                    } else {
+                        T e[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) e[k] = q[k];
+                        memcpy(&v[u], e, 16);
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < QB; u++) {
+                const int i = i0 + u * THREADS, rr = i / W, c = i % W;
+                if (i < 256 * W) st_shared16(sK + rr * (2 * HD) + ((c ^ (rr & 3)) << 4), v[u].x, v[u].y, v[u].z, v[u].w);
+            }
+        }
+        __syncthreads();
         float f = 0.0f;                         // of this row's scores, in log2 units
         int lim = 0;                            // keys this row sees
         const int col = c0 + threadIdx.x;
         const int row = rq.row0 + (warp < SOFT && col < n_cols ? col / G : 0), head = kh * G + (col < n_cols ? col % G : 0);
         if (warp < SOFT) {
             const bool there = col < n_cols;
-            const T * q = (const T *) a.q + (long long) row * a.q_tok + head * a.q_head;
-            auto word = [&](int s, float (&x)[8]) {
-                const T * p = q + 32 * (s % NG) + 8 * (s / NG);
+            const uint32_t mine = sK + threadIdx.x * (2 * HD);
+            auto word = [&](int s, float (&x)[8]) {         // words in the order of the key rows
                 T e[8];
-                if (!there) {
-#pragma unroll
-                    for (int c = 0; c < 8; c++) e[c] = to_type<T>(0.0f);
-                } else if (vec & 1) {
-                    *(uint4 *) e = *(const uint4 *) p;
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 8; c++) e[c] = p[c];
-                }
+                const uint4 v = ld_shared16(mine + (((4 * (s % NG) + s / NG) ^ (lane & 3)) << 4));
+                memcpy(e, &v, 16);
 #pragma unroll
                 for (int c = 0; c < 8; c++) x[c] = from_type(e[c]);
             };
@@ -259,37 +285,36 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
             // this head's rows and scales of page 0, and from page to page
             const uint32_t d_plane = ((uint32_t) pool.heads * NG) << pool.page_shift, q_page = ((uint32_t) pool.heads << pool.page_shift) * 32 * NG;
             const uint8_t * q_head = pool.q + kv4_q_at(pool, 0, keys ? 0 : 1, kh, 0);
-            const __half * d_head = pool.d + kv4_d_at(pool, 0, keys ? 0 : 1, kh, 0);
-            auto page_at = [&](int key) -> int {
-                const int p = key < kend ? __ldg(table + (key >> pool.page_shift)) : -1;
-                return p < n_pages ? p : -1;
-            };
+            const uint16_t * d_head = (const uint16_t *) pool.d + kv4_d_at(pool, 0, keys ? 0 : 1, kh, 0);
+            // (a table entry is loaded a block before it is used and checked: volatile, or the compiler puts the load off to
+            // its use, and the block waits for it)
+            auto entry_at = [&](int key) -> int { return key < kend ? *(const volatile int32_t *) (table + (key >> pool.page_shift)) : -1; };
             uint4 raw[NG], next[NG];                            // this block's row and the next one's
-            __half d[NG], dn[NG], vd[NG], vdn[NG];              // their scales (vd, K warps: those of the value, for the masks)
-            int page = page_at(k0 + kt), heldn = -1;            // of the block to be loaded; of the one in `next`
+            // their scales (vd, K warps: those of the value, for the masks); in 32 bits each: pairs of 16 would be put
+            // together, and waited for, as soon as they are loaded
+            uint32_t d[NG], dn[NG], vd[NG], vdn[NG];
+            int entry = entry_at(k0 + kt), heldn = -1;          // table entry of the block to be loaded; page of the one in `next`
             auto load = [&](int j) {
                 const int key = k0 + j * BLK + kt;
+                const int page = (uint32_t) entry < (uint32_t) n_pages ? entry : -1;
                 heldn = page;
-                if (page >= 0) {
-                    const uint4 * q = (const uint4 *) (q_head + (uint64_t) (uint32_t) page * q_page + (key & pmask) * 16 * NG);
-                    const __half * s = d_head + (uint64_t) (uint32_t) page * (2 * d_plane) + (key & pmask);
+                // (a row without a page loads page 0's, and its scales become 0 at its use: a branch, or a choice of values
+                // here, would wait for the loads)
+                const uint4 * q = (const uint4 *) (q_head + (uint64_t) (uint32_t) max(page, 0) * q_page + (key & pmask) * 16 * NG);
+                const uint16_t * s = d_head + (uint64_t) (uint32_t) max(page, 0) * (2 * d_plane) + (key & pmask);
 #pragma unroll
-                    for (int i = 0; i < NG; i++) next[i] = q[i];
+                for (int i = 0; i < NG; i++) next[i] = q[i];
 #pragma unroll
-                    for (int i = 0; i < NG; i++) { dn[i] = s[i * P]; if (keys) vdn[i] = s[d_plane + i * P]; }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < NG; i++) { next[i] = make_uint4(0, 0, 0, 0); dn[i] = vdn[i] = __ushort_as_half(0); }
-                }
-                if (j + 1 < nb_all) page = page_at(key + BLK);
+                for (int i = 0; i < NG; i++) { dn[i] = s[i * P]; vdn[i] = s[(keys ? d_plane : 0) + i * P]; }
+                if (j + 1 < nb_all) entry = entry_at(key + BLK);
             };
             if (nb_all > 0) load(0);
             bool ok = true;
             for (int j = 0; j < nb_all; j++) {
                 const int s = j % STAGES, slot = j % SLOTS;
-                const bool hole = heldn < 0 && k0 + j * BLK + kt < kend;
+                const bool live = heldn >= 0, hole = !live && k0 + j * BLK + kt < kend;
 #pragma unroll
-                for (int i = 0; i < NG; i++) { raw[i] = next[i]; d[i] = dn[i]; vd[i] = vdn[i]; }
+                for (int i = 0; i < NG; i++) { raw[i] = next[i]; d[i] = live ? dn[i] : 0; vd[i] = live ? vdn[i] : 0; }
                 if (j + 1 < nb_all) load(j + 1);
                 // block j - STAGES, which had this stage, is done with in every tile that took it
                 if (j >= STAGES) {
@@ -304,7 +329,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                     uint32_t any = holes;
 #pragma unroll
                     for (int i = 0; i < NG; i++) {
-                        const uint32_t m = __ballot_sync(0xffffffffu, __hisnan(vd[i]) || __hisinf(vd[i]));
+                        const uint32_t m = __ballot_sync(0xffffffffu, not_finite(vd[i]));
                         any |= m;
                         if (lane == 0) s_bad[slot][i][cw] = m;
                     }
@@ -312,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                 } else {
 #pragma unroll
                     for (int i = 0; i < NG; i++) {
-                        if (__hisnan(d[i]) || __hisinf(d[i])) d[i] = __ushort_as_half(0);
+                        if (not_finite(d[i])) d[i] = 0;
                     }
                 }
                 const uint32_t dst = (keys ? sK : sV) + s * AT * ATOM + kt * 128;
@@ -320,7 +345,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                 for (int i = 0; i < W; i++) {
                     const uint4 & q4 = raw[i / 4];
                     const uint32_t w = (i & 3) == 0 ? q4.x : (i & 3) == 1 ? q4.y : (i & 3) == 2 ? q4.z : q4.w;
-                    const __half2 d2 = __half2half2(keys ? d[i % NG] : d[i / 4]);       // a key row's groups take turns
+                    const __half2 d2 = u2h((keys ? d[i % NG] : d[i / 4]) * 0x10001u);     // a key row's groups take turns
                     __half2 x[4];
                     codes4(w, x);
                     st_shared16(dst + (i / 8) * ATOM + (((i & 7) ^ (kt & 7)) << 4), h2u(__hmul2(x[0], d2)), h2u(__hmul2(x[1], d2)),
