@@ -68,23 +68,25 @@ __device__ __forceinline__ __half group_scale(float hi, float lo) {
     return finite ? __float2half_rn(d) : __ushort_as_half((unsigned short) 0x7fff);
 }
 
-// code = clamp(floor(x / d + 1/2) + 8, 0, 15).
+// 2^23 + code in the bits of a float, code = clamp(floor(x / d + 1/2) + 8, 0, 15); inv is 1 / d within 2^-23 of itself.
 // For f16 and bf16 x the quotient of an 11-bit by an 8-bit significand is a half-integer or at least 2^-13 away
 // from one (for |quotient| between 1/2 and 8.1), and x * inv is within 2^-19 of it: adding 2^-15 decides every case as the
-// exact quotient would. For f32 x the estimate is corrected by the sign of x - (c -+ 1/2) d, one fused rounding each.
+// exact quotient would. The clamp is the saturation of (quotient + 8.5) / 16 to [0, 1], and the factor a step below 16
+// sends 1 to 15 (it moves the rest by 2^-20 at most). For f32 x the estimate is corrected by the sign of
+// x - (c -+ 1/2) d, one fused rounding each.
 template <class T>
-__device__ __forceinline__ uint32_t code_of(float x, float d, float inv) {
-    float t = __fmaf_rn(x, inv, 8.5f + 0x1p-15f);
-    t = fminf(fmaxf(t, 0.0f), 15.5f);
-    uint32_t c = __float_as_uint(__fadd_rd(t, 8388608.0f)) & 15u;   // floor, in the low bits of 2^23 + t
+__device__ __forceinline__ uint32_t code_of(float x, float d, float inv16) {
+    const float t = __saturatef(__fmaf_rn(x, inv16, (8.5f + 0x1p-15f) * 0.0625f));
+    uint32_t u = __float_as_uint(__fmaf_rd(t, 15.999999f, 8388608.0f));
     if (sizeof(T) == 4) {
+        const uint32_t c = u & 15u;
         const float s = d < 0.0f ? -1.0f : 1.0f;
         const float k = (float) c - 8.0f;
         const float below = __fmaf_rn(-(k - 0.5f), d, x) * s, above = __fmaf_rn(-(k + 0.5f), d, x) * s;
-        if (below < 0.0f && c > 0) c--;
-        else if (above >= 0.0f && c < 15) c++;
+        if (below < 0.0f && c > 0) u--;
+        else if (above >= 0.0f && c < 15) u++;
     }
-    return c;
+    return u;
 }
 
 template <class T, int NG>
@@ -104,11 +106,14 @@ __device__ __forceinline__ void quantise_row(const Vec8<T> (&in)[NG], uint32_t (
         scale[g] = group_scale(hi, lo);
         const float d = __half2float(scale[g]);
         const bool zero = d == 0.0f || d != d;
-        const float inv = zero ? 0.0f : __fdiv_rn(1.0f, d);
+        float inv;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(zero ? 1.0f : d));
+        inv *= 0.0625f;
+        // the codes' words add up with weights 16^i; the 2^23 that each carries adds up to 0xfb000000 modulo 2^32
         uint32_t w = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) w |= code_of<T>(x[i], d, inv) << (4 * i);
-        word[g] = zero ? 0x88888888u : w;
+        for (int i = 7; i >= 0; i--) w = w * 16u + code_of<T>(x[i], d, inv);
+        word[g] = zero ? 0x88888888u : w - 0xfb000000u;
     }
 }
 
