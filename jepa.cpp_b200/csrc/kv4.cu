@@ -285,33 +285,7 @@ int kv4_load(const Kv4Pool & p, const Kv4Rows & r, int type, const int64_t * slo
 
 namespace {
 
-constexpr int TAB_THREADS = 512;
-
-struct TokPg { long long tok, pg; };
-
-// inclusive scan over the block of one pair per thread; `total` receives the block's sums
-__device__ __forceinline__ TokPg block_scan(TokPg x, TokPg & total, TokPg * warp_sum) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long a = __shfl_up_sync(0xffffffffu, x.tok, o), b = __shfl_up_sync(0xffffffffu, x.pg, o);
-        if (lane >= o) { x.tok += a; x.pg += b; }
-    }
-    __syncthreads();                     // the array's last readers are done
-    if (lane == 31) warp_sum[warp] = x;
-    __syncthreads();
-    TokPg before = {0, 0};
-    total = {0, 0};
-    for (int w = 0; w < nw; w++) {
-        const TokPg s = warp_sum[w];
-        if (w < warp) { before.tok += s.tok; before.pg += s.pg; }
-        total.tok += s.tok;
-        total.pg += s.pg;
-    }
-    x.tok += before.tok;
-    x.pg += before.pg;
-    return x;
-}
+constexpr int TAB_THREADS = 512, TAB_RUN = 4;       // requests a thread takes at a time, in a row
 
 struct Request { int cached, added, held, need, bad; };
 
@@ -340,40 +314,52 @@ __device__ __forceinline__ int last_le(const int * v, int n, int x) {
     return lo;
 }
 
-// Every CTA walks all requests, TAB_THREADS a time, with a scan of their new tokens and new pages (two integers a
-// request: it stays in L2), and writes its own share of the flat outputs: slots and fresh table entries, each found by
-// bisection among the walked requests' first tokens / pages. One launch, no communication between CTAs, balanced however
-// unequal the requests are. A refused step (state[0] != 0) is known to every CTA before anything is written.
+// Every CTA walks all requests, 4 a thread at a time: first their totals (in 64 bits), which decide whether the step is
+// refused before anything is written, then a scan of new tokens and new pages, and writes its own share of the flat
+// outputs: slots and fresh table entries, each found by bisection among the walked requests' first tokens / pages. One
+// launch, no communication between CTAs, balanced however unequal the requests are; the lengths (8 bytes a
+// request) stay in L2. What it costs is latency: two loads, two block sums and a bisection (4000 requests and 517,000 slots in
+// 148 CTAs: 8 walks of 512 requests with two 64-bit scans took 22 us).
 __global__ void __launch_bounds__(TAB_THREADS) k_kv_tables(const KvTablesArgs a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    __shared__ TokPg warp_sum[TAB_THREADS / 32];
-    __shared__ int first_tok[TAB_THREADS], first_pg[TAB_THREADS], s_cached[TAB_THREADS], s_held[TAB_THREADS];
-    __shared__ int s_bad;
-    const int tid = threadIdx.x, nt = blockDim.x;
-    const int n_chunks = (a.n_req + nt - 1) / nt;
-    if (tid == 0) s_bad = 0x7fffffff;
-    __syncthreads();
-    // totals and refusals (one chunk: the scan below gives them)
-    TokPg all = {0, 0};
-    Request q = request_of(a, tid);
-    {
-        TokPg mine = {q.added, q.need};
-        int bad = q.bad ? q.bad : 0x7fffffff;
-        for (int r = tid + nt; r < a.n_req; r += nt) {
-            const Request o = request_of(a, r);
-            mine.tok += o.added;
-            mine.pg += o.need;
+    __shared__ int first_tok[TAB_THREADS * TAB_RUN], first_pg[TAB_THREADS * TAB_RUN], s_cached[TAB_THREADS * TAB_RUN];
+    __shared__ long long w_tok[TAB_THREADS / 32], w_pg[TAB_THREADS / 32];
+    __shared__ int2 w_sum[TAB_THREADS / 32];
+    __shared__ int w_bad[TAB_THREADS / 32];
+    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, nw = nt >> 5, run = nt * TAB_RUN;
+    const int n_chunks = (a.n_req + run - 1) / run, P1 = (1 << a.page_shift) - 1;
+    // totals and refusals; the first chunk's requests stay in registers
+    Request q[TAB_RUN];
+    long long tok = 0, pg = 0;
+    int bad = 0x7fffffff;
+#pragma unroll
+    for (int k = 0; k < TAB_RUN; k++) q[k] = request_of(a, tid * TAB_RUN + k);
+#pragma unroll
+    for (int k = 0; k < TAB_RUN; k++) { tok += q[k].added; pg += q[k].need; if (q[k].bad) bad = min(bad, q[k].bad); }
+    for (int c = 1; c < n_chunks; c++) {
+#pragma unroll
+        for (int k = 0; k < TAB_RUN; k++) {
+            const Request o = request_of(a, c * run + tid * TAB_RUN + k);
+            tok += o.added;
+            pg += o.need;
             if (o.bad) bad = min(bad, o.bad);
         }
-        if (bad != 0x7fffffff) atomicMin(&s_bad, bad);
-        block_scan(mine, all, warp_sum);
     }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        tok += __shfl_xor_sync(0xffffffffu, tok, o);
+        pg += __shfl_xor_sync(0xffffffffu, pg, o);
+    }
+    bad = __reduce_min_sync(0xffffffffu, bad);
+    if (lane == 0) { w_tok[warp] = tok; w_pg[warp] = pg; w_bad[warp] = bad; }
     __syncthreads();
-    int status = s_bad == 0x7fffffff ? 0 : s_bad;
-    if (!status && all.pg > a.n_free) status = 3;
-    if (!status && all.tok > a.n_slots) status = 4;
-    const int n_tok = status ? 0 : (int) all.tok, n_pg = status ? 0 : (int) all.pg;
+    tok = pg = 0;
+    for (int w = 0; w < nw; w++) { tok += w_tok[w]; pg += w_pg[w]; bad = min(bad, w_bad[w]); }
+    int status = bad == 0x7fffffff ? 0 : bad;
+    if (!status && pg > a.n_free) status = 3;
+    if (!status && tok > a.n_slots) status = 4;
+    const int n_tok = status ? 0 : (int) tok, n_pg = status ? 0 : (int) pg;
     if (blockIdx.x == 0 && tid == 0) {
         a.state[0] = status;
         a.state[1] = n_pg;
@@ -382,33 +368,59 @@ __global__ void __launch_bounds__(TAB_THREADS) k_kv_tables(const KvTablesArgs a)
     const int s0 = (int) ((long long) a.n_slots * blockIdx.x / gridDim.x), s1 = (int) ((long long) a.n_slots * (blockIdx.x + 1) / gridDim.x);
     const int p0 = (int) ((long long) n_pg * blockIdx.x / gridDim.x), p1 = (int) ((long long) n_pg * (blockIdx.x + 1) / gridDim.x);
     for (int i = max(s0, n_tok) + tid; i < s1; i += nt) a.slots[i] = -1;
-    int tok0 = 0, pg0 = 0;                // first token and page of the chunk
+    int tok0 = 0, pg0 = 0;                // first token and page of the chunk (32 bits hold what is not refused)
     for (int c = 0; c < n_chunks; c++) {
-        const int r0 = c * nt, r = r0 + tid, n = min(nt, a.n_req - r0);
-        if (c) q = request_of(a, r);
+        const int r0 = c * run, n = min(run, a.n_req - r0);
+        const bool mine = c % gridDim.x == blockIdx.x;       // this CTA writes the chunk's lens and q_start
         if (status) {
-            if (c % gridDim.x == blockIdx.x && r < a.n_req) { a.lens[r] = a.cached[r]; a.q_start[r] = 0; }
+            if (mine) {
+                for (int i = tid; i < n; i += nt) { a.lens[r0 + i] = a.cached[r0 + i]; a.q_start[r0 + i] = 0; }
+            }
             continue;
         }
-        TokPg sum;
-        const TokPg inc = block_scan({q.added, q.need}, sum, warp_sum);
-        first_tok[tid] = tok0 + (int) inc.tok - q.added;
-        first_pg[tid] = pg0 + (int) inc.pg - q.need;
-        s_cached[tid] = q.cached;
-        s_held[tid] = q.held;
-        if (c % gridDim.x == blockIdx.x && r < a.n_req) { a.lens[r] = q.cached + q.added; a.q_start[r] = first_tok[tid]; }
+        if (c) {
+#pragma unroll
+            for (int k = 0; k < TAB_RUN; k++) q[k] = request_of(a, r0 + tid * TAB_RUN + k);
+        }
+        int2 own = make_int2(0, 0);
+#pragma unroll
+        for (int k = 0; k < TAB_RUN; k++) { own.x += q[k].added; own.y += q[k].need; }
+        int2 inc = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, inc.x, o), y = __shfl_up_sync(0xffffffffu, inc.y, o);
+            if (lane >= o) { inc.x += x; inc.y += y; }
+        }
+        if (lane == 31) w_sum[warp] = inc;
         __syncthreads();
-        const int tok1 = tok0 + (int) sum.tok, pg1 = pg0 + (int) sum.pg;
+        int t = tok0 + inc.x - own.x, g = pg0 + inc.y - own.y, tok1 = tok0, pg1 = pg0;
+        for (int w = 0; w < nw; w++) {
+            const int2 s = w_sum[w];
+            if (w < warp) { t += s.x; g += s.y; }
+            tok1 += s.x;
+            pg1 += s.y;
+        }
+#pragma unroll
+        for (int k = 0; k < TAB_RUN; k++) {
+            const int i = tid * TAB_RUN + k;
+            first_tok[i] = t;
+            first_pg[i] = g;
+            s_cached[i] = q[k].cached;
+            if (mine && i < n) { a.lens[r0 + i] = q[k].cached + q[k].added; a.q_start[r0 + i] = t; }
+            t += q[k].added;
+            g += q[k].need;
+        }
+        __syncthreads();
         for (int i = max(p0, pg0) + tid; i < min(p1, pg1); i += nt) {
             const int k = last_le(first_pg, n, i);
-            a.table[(size_t) (r0 + k) * a.width + s_held[k] + (i - first_pg[k])] = a.free_pages[i];
+            a.table[(size_t) (r0 + k) * a.width + ((s_cached[k] + P1) >> a.page_shift) + (i - first_pg[k])] = a.free_pages[i];
         }
         for (int i = max(s0, tok0) + tid; i < min(s1, tok1); i += nt) {
             const int k = last_le(first_tok, n, i);
-            const int pos = s_cached[k] + (i - first_tok[k]), idx = pos >> a.page_shift;
+            const int pos = s_cached[k] + (i - first_tok[k]), idx = pos >> a.page_shift, held = (s_cached[k] + P1) >> a.page_shift;
             // a page held before this step comes from the table, a fresh one from the free list
-            const int page = idx < s_held[k] ? a.table[(size_t) (r0 + k) * a.width + idx] : a.free_pages[first_pg[k] + idx - s_held[k]];
-            a.slots[i] = page < 0 ? -1 : ((long long) page << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+            const int page = idx < held ? a.table[(size_t) (r0 + k) * a.width + idx] : a.free_pages[first_pg[k] + idx - held];
+            a.slots[i] = page < 0 ? -1 : ((long long) page << a.page_shift) + (pos & P1);
         }
         tok0 = tok1;
         pg0 = pg1;
