@@ -86,6 +86,12 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// all threads of the CTA, from any branch
+__device__ __forceinline__ void cta_sync() {
+    fence_before();
+    asm volatile("barrier.sync 0;" ::: "memory");
+    fence_after();
+}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -179,11 +185,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
         const int nb_all = kend > k0 ? (kend - k0 + BLK - 1) / BLK : 0;
         const int kend0 = n_tiles == 1 ? kend : min(visible(rq, rq.row0 + (c0 + 127) / G, a.frame), kend);
         const int nb0 = kend0 > k0 ? (kend0 - k0 + BLK - 1) / BLK : 0;          // blocks of tile 0
-        fence_before();
-        __syncthreads();                        // TMEM is there, and free of the columns before
-        fence_after();
-        const uint32_t tmem = tmem_sh;
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == THREADS - 1) {
             for (int s = 0; s < STAGES; s++) {
                 mbar_init(&bars.k_full[s], CONV / 2);
                 mbar_init(&bars.v_full[s], CONV / 2);
@@ -198,6 +200,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                 }
             }
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            fence_async();
         }
         // ---- queries: first as they are into the stages' memory, by consecutive threads along the rows (a thread a row took
         // 32 cache lines a load, 8,000 to 15,000 cycles in all), then thread = row of the tiles
@@ -226,7 +229,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                 if (i < 256 * W) st_shared16(sK + rr * (2 * HD) + ((c ^ (rr & 3)) << 4), v[u].x, v[u].y, v[u].z, v[u].w);
             }
         }
-        __syncthreads();
+        cta_sync();                             // TMEM is there, and free of the columns before
+        const uint32_t tmem = tmem_sh;
         float f = 0.0f;                         // of this row's scores, in log2 units
         int lim = 0;                            // keys this row sees
         const int col = c0 + threadIdx.x;
@@ -270,11 +274,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                 if (QT) tmem_st16(qc + 4 * s, w);
             }
             tmem_wait_st();
-            fence_async();                      // (the barriers)
+            fence_async();                      // queries in shared memory
         }
-        fence_before();
-        __syncthreads();
-        fence_after();
 
         if (warp >= SOFT && warp < SOFT + CONV) {
             // ---- conversion: thread = a K row (warps 8, 9) or a V row (10, 11) of the block
@@ -309,6 +310,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                 if (j + 1 < nb_all) entry = entry_at(key + BLK);
             };
             if (nb_all > 0) load(0);
+            cta_sync();                         // the queries have left the stages' memory
             bool ok = true;
             for (int j = 0; j < nb_all; j++) {
                 const int s = j % STAGES, slot = j % SLOTS;
@@ -358,6 +360,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
             if (!ok) abort_sh = 1;
         } else if (warp >= SOFT + CONV) {
             // ---- products of tile t: the whole warp waits, one lane issues
+            cta_sync();                         // the queries are in place
             const int t = warp - SOFT - CONV, nb = t == 0 ? nb0 : t < n_tiles ? nb_all : 0;
             const uint32_t q_desc = (uint32_t) sw128_desc(sQ + t * AT * QATOM), k_desc = (uint32_t) sw128_desc(sK), v_desc = (uint32_t) mn_desc(sV), hi = (uint32_t) (sw128_desc(0) >> 32);
             const uint32_t od = tmem + HD * t, qd = tmem + Q_COL + HD / 2 * t, sd = tmem + S_COL + NB * BLK * t;
@@ -410,6 +413,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
             if (!ok) abort_sh = 1;
         } else if (128 * (warp >> 2) + 32 * (warp & 3) < cols) {
             // ---- softmax: thread = row
+            cta_sync();
             const int t = warp >> 2, nb = t == 0 ? nb0 : nb_all;
             const uint32_t lanes = (uint32_t) (32 * (warp & 3)) << 16;
             const uint32_t ts = tmem + lanes + S_COL + NB * BLK * t, to = tmem + lanes + HD * t;
@@ -595,9 +599,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
             }
             if (there && used > 1) sp.ml[at] = make_float2(z, l);
         }
-        fence_before();
-        __syncthreads();
-        fence_after();
+        else {
+            cta_sync();                         // a softmax warp without rows
+        }
+        cta_sync();
         if (*(volatile int *) &abort_sh) break;
         if (threadIdx.x == 0) {                 // the next columns start with fresh barriers
             for (int i = 0; i < (int) (sizeof(Bars) / 8); i++) {
