@@ -180,7 +180,7 @@ int jepa_b200_kv4_bytes(const jepa_b200_kv4_cache * cache, size_t * q_bytes, siz
 //                         outgrows its table row (or 2^31), 3 too few free pages, 4 more than n_slots new rows
 // A refused step (the smallest code of those that apply) leaves `table` as it was, sets lens = cached, q_start = 0 and
 // slots = -1, so that the calls behind it store and compute nothing. Table entries behind the taken pages stay as
-// they were. The arrays must not overlap. n_req, width, n_slots >= 1.
+// they were. The arrays must not overlap. n_req, width, n_slots >= 1; n_req, n_slots, n_free <= 2^30.
 int jepa_b200_kv_tables(const int32_t * cached, const int32_t * added, int n_req, int page_size, int32_t * table, int width,
                         const int32_t * free_pages, int n_free, int32_t * lens, int32_t * q_start, int64_t * slots, int n_slots,
                         int32_t * state, void * stream);
@@ -213,7 +213,7 @@ typedef struct jepa_b200_kv4_attn {
     const int32_t * lens;     // [n_req]
     const int32_t * table;    // [n_req][width]
     int32_t n_req;            // 0 .. 65535
-    int32_t n_rows;           // rows of q and out
+    int32_t n_rows;           // rows of q and out (n_rows * n_heads <= 2^30)
     int32_t width;
     int32_t n_heads;          // a multiple of kv_heads
     uint32_t type;            // 1 (f16) or 30 (bf16)
@@ -226,6 +226,11 @@ typedef struct jepa_b200_kv4_attn {
 } jepa_b200_kv4_attn;
 int64_t jepa_b200_kv4_attention_workspace(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args);
 int jepa_b200_kv4_attention(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, void * stream);
+
+// Waits for `stream` and reports (and clears) the failure flag of the attention's bounded device waits on the current
+// device: 0, or -1 with the reason when a kernel gave up on its pipeline (its rows are NaN then). Not for a capturing
+// stream.
+int jepa_b200_kv4_check(void * stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

@@ -73,5 +73,6 @@ struct Kv4Attn {
 };
 size_t kv4_attention_workspace(const Kv4Pool & p, const Kv4Attn & a);
 int kv4_attention(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st);
+int kv4_error_flag(cudaStream_t st);            // waits for the stream; reads and resets: 0, or the wait that ran out (-1: not read)
 
 }  // namespace jb

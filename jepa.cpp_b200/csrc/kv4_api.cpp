@@ -68,6 +68,7 @@ bool attn_of(const char * fn, const jb::Kv4Pool & p, const jepa_b200_kv4_attn * 
         return false;
     }
     if (((long long) x->width << p.page_shift) > 0x7fffffffLL - 1024) { log("jepa: %s: %d table columns exceed 2^31 positions\n", fn, x->width); return false; }
+    if ((long long) x->n_rows * x->n_heads > (1 << 30)) { log("jepa: %s: %d rows of %d heads are more than 2^30\n", fn, x->n_rows, x->n_heads); return false; }
     if (x->frame < 0 || x->max_len < 0 || x->max_new < 0) { log("jepa: %s: frame %d, max_len %d and max_new %d must not be negative\n", fn, x->frame, x->max_len, x->max_new); return false; }
     if (!std::isfinite(x->scale)) { log("jepa: %s: scale is not finite\n", fn); return false; }
     if (x->q_tok < 0 || x->q_head < 0 || x->o_tok < 0 || x->o_head < 0) { log("jepa: %s: strides must not be negative\n", fn); return false; }
@@ -109,8 +110,9 @@ int jepa_b200_kv_tables(const int32_t * cached, const int32_t * added, int n_req
                         const int32_t * free_pages, int n_free, int32_t * lens, int32_t * q_start, int64_t * slots, int n_slots,
                         int32_t * state, void * stream) {
     static const char * fn = "jepa_b200_kv_tables";
-    if (n_req < 1 || width < 1 || n_free < 0 || n_slots < 1) {
-        log("jepa: %s: need n_req, width and n_slots of 1 or more and n_free of 0 or more (%d, %d, %d, %d)\n", fn, n_req, width, n_slots, n_free);
+    constexpr int MAX = 1 << 30;        // of each count: the kernel's 32-bit indices step past the end by less than that
+    if (n_req < 1 || width < 1 || n_free < 0 || n_slots < 1 || n_req > MAX || n_free > MAX || n_slots > MAX) {
+        log("jepa: %s: need n_req, width and n_slots of 1 or more, n_free of 0 or more, none above 2^30 (%d, %d, %d, %d)\n", fn, n_req, width, n_slots, n_free);
         return -1;
     }
     if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1))) {
@@ -174,6 +176,12 @@ int jepa_b200_kv4_attention(const jepa_b200_kv4_cache * cache, const jepa_b200_k
     if (device_pointers(fn, {{"cache.q", p.q, 16}, {"cache.d", p.d, 16}, {"q", a.q, 2}, {"out", a.out, 2}, {"q_start", a.q_start, 4},
                              {"lens", a.lens, 4}, {"table", a.table, 4}, {"workspace", ws, 16}})) return -1;
     return jb::kv4_attention(p, a, (cudaStream_t) stream);
+}
+
+int jepa_b200_kv4_check(void * stream) {
+    const int code = jb::kv4_error_flag((cudaStream_t) stream);
+    if (code > 0) log("jepa: jepa_b200_kv4_check: an attention kernel gave up waiting on its pipeline (wait %d); its rows are NaN\n", code);
+    return code == 0 ? 0 : -1;
 }
 
 }  // extern "C"

@@ -93,8 +93,8 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
     const Req rq = request_of(a, pool.page_shift, r);
     const int n_cols = (rq.row1 - rq.row0) * G;              // (token, head of the group) columns of this cache head
     const int span = sp.span(rq.len), used = sp.used(rq.len);
-    const int k0 = blockIdx.x * span, k1 = min(rq.len, k0 + span);
     if (n_cols <= 0 || (blockIdx.x && (int) blockIdx.x >= used)) return;
+    const int k0 = blockIdx.x * span, k1 = range_end(rq.len, k0, span);
     const int32_t * table = a.table + (size_t) r * a.width;
     const int n_pages = (int) (pool.n_slots >> pool.page_shift), pmask = (1 << pool.page_shift) - 1;
     uint8_t * ring = smem + warp * STAGES * SB;
@@ -551,7 +551,8 @@ int launch(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st) {
     if (r.tc && kv4_tiles(p, a, r.sp, r.tiles, vec, st)) return -1;
     if (r.nt == 1 ? rows_launch<T, NG, 1>(p, a, r, vec, st) : rows_launch<T, NG, 2>(p, a, r, vec, st)) return -1;
     if (r.sp.n_split > 1) {
-        const dim3 grid((unsigned) std::max(1, a.max_new), (unsigned) a.heads, (unsigned) a.n_req);
+        // (a CTA walks rows of its request from its own on: max_new may be unknown, and then far too many)
+        const dim3 grid((unsigned) std::min(std::max(1, a.max_new), 64), (unsigned) a.heads, (unsigned) a.n_req);
         JB_CUDA(launch_pdl(k_kv4_merge<T, NG>, grid, dim3(256), 0, st, p, a, r.sp));
     }
     return 0;

@@ -170,8 +170,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
     const Req rq = request_of(a, pool.page_shift, r);
     const int n_cols = tile_columns((rq.row1 - rq.row0) * G);
     const int span = sp.span(rq.len), used = sp.used(rq.len);
-    const int k0 = blockIdx.x * span;
     if (n_cols <= 0 || (int) (blockIdx.y % tiles) * 256 >= n_cols || (blockIdx.x && (int) blockIdx.x >= used)) return;
+    const int k0 = blockIdx.x * span, k1 = range_end(rq.len, k0, span);
 
     if (warp == SOFT) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&tmem_sh)), "r"(512) : "memory");
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
 
     for (int c0 = (int) (blockIdx.y % tiles) * 256; c0 < n_cols; c0 += tiles * 256) {
         const int cols = min(256, n_cols - c0), n_tiles = cols > 128 ? 2 : 1;
-        const int kend = min(visible(rq, rq.row0 + (c0 + cols - 1) / G, a.frame), min(rq.len, k0 + span));   // the last row sees most
+        const int kend = min(visible(rq, rq.row0 + (c0 + cols - 1) / G, a.frame), k1);   // the last row sees most
         const int nb_all = kend > k0 ? (kend - k0 + BLK - 1) / BLK : 0;
         const int kend0 = n_tiles == 1 ? kend : min(visible(rq, rq.row0 + (c0 + 127) / G, a.frame), kend);
         const int nb0 = kend0 > k0 ? (kend0 - k0 + BLK - 1) / BLK : 0;          // blocks of tile 0
@@ -635,6 +635,17 @@ int launch_dim(const Kv4Pool & p, const Kv4Attn & a, const Split & sp, int tiles
 }
 
 }  // namespace
+
+int kv4_error_flag(cudaStream_t st) {
+    int v = 0;
+    static const int zero = 0;
+    if (!cuda_ok(cudaMemcpyFromSymbolAsync(&v, g_kv4_error, sizeof(int), 0, cudaMemcpyDeviceToHost, st), "reading the 4-bit cache's error flag") ||
+        !cuda_ok(cudaMemcpyToSymbolAsync(g_kv4_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st), "resetting the 4-bit cache's error flag") ||
+        !cuda_ok(cudaStreamSynchronize(st), "reading the 4-bit cache's error flag")) {
+        return -1;
+    }
+    return v;
+}
 
 int kv4_tiles(const Kv4Pool & p, const Kv4Attn & a, const Split & sp, int tiles, int vec, cudaStream_t st) {
     return a.type == KV4_F16 ? launch_dim<__half>(p, a, sp, tiles, vec, st) : launch_dim<__nv_bfloat16>(p, a, sp, tiles, vec, st);

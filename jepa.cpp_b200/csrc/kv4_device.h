@@ -35,6 +35,9 @@ struct Split {
     __host__ __device__ int used(int len) const { return len > 0 ? (len - 1) / span(len) + 1 : 0; }
 };
 
+// end of the range of `span` keys that starts at k0 (k0 + span may pass 2^31)
+__device__ __forceinline__ int range_end(int len, int k0, int span) { return len - k0 < span ? len : k0 + span; }
+
 // What a CTA needs to know of its request: rows [row0, row1) of q, keys [0, len) of the table.
 struct Req {
     int row0, row1, last, len, lens;

@@ -48,6 +48,7 @@ def _load() -> C.CDLL:
             "jepa_b200_kv4_load": (i32, [cp, vp, i64, vp, vp, C.c_uint32, vp]),
             "jepa_b200_kv4_attention_workspace": (i64, [cp, C.POINTER(_Attn)]),
             "jepa_b200_kv4_attention": (i32, [cp, C.POINTER(_Attn), vp]),
+            "jepa_b200_kv4_check": (i32, [vp]),
         }
         for name, (res, args) in sig.items():
             f = getattr(L, name)
@@ -112,7 +113,7 @@ def build_tables(cached: torch.Tensor, added: torch.Tensor, table: torch.Tensor,
     _index(free_pages, "free_pages", torch.int32, dev)
     _need(added.shape[0] == n and table.shape[0] == n, "cached, added and table must have one entry a request")
     _need(n >= 1 and table.shape[1] >= 1, "there must be a request and a table column")
-    _need(1 <= n_slots < 2 ** 31, f"n_slots {n_slots} is not 1 .. 2^31 - 1")
+    _need(max(n, table.shape[1], free_pages.shape[0], n_slots, page_size) <= 2 ** 30, "no count may pass 2^30")
     # lens, q_start and state share one allocation, each at a multiple of 4 bytes
     ints = torch.empty(2 * n + 3, dtype=torch.int32, device=dev)
     lens, q_start, state = ints.split((n, n + 1, 2))
@@ -209,6 +210,8 @@ class KV4Cache:
         n, width = table.shape
         if q_start.shape[0] != n + 1 or lens.shape[0] != n:
             raise ValueError("lens, q_start and table must agree on the requests")
+        if max(rows, n, width, frame, max_len, max_new) >= 2 ** 31:
+            raise ValueError("no count may pass 2^31 - 1")
         if out is None:
             out = torch.zeros((rows, heads, self.head_dim), dtype=q.dtype, device=self._dev)
         elif out.dtype is not q.dtype:
@@ -228,3 +231,7 @@ class KV4Cache:
             a.workspace, a.workspace_bytes = ws.data_ptr(), need
         _call("jepa_b200_kv4_attention", self._dev, self._ref, ref)
         return out
+
+    def check(self) -> None:
+        """Waits for the current stream; raises if an attention kernel on it gave up waiting (its rows are NaN)."""
+        _call("jepa_b200_kv4_check", self._dev)

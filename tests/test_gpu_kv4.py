@@ -308,6 +308,9 @@ CASES = [
     ([50, 60], [64, 61], 4, 2, 64, 16, 1),       # more rows than keys: the first rows see nothing
     ([20], [150], 7, 1, 128, 16, 16),
     ([1000, 0, 129, 128, 127], [130, 3, 129, 1, 0], 8, 4, 64, 128, 1),
+    ([90, 300], [1, 1], 512, 1, 64, 16, 1),      # more columns of one row than a tile holds
+    ([70, 20, 200], [3, 1, 6], 86, 1, 128, 32, 1),   # 258, 86 and 516 columns: whole tiles and 2, 86 and 4 left over
+    ([640, 64, 900], [1, 64, 2], 4, 1, 96, 64, 0),   # single rows beside a chunk
 ]
 
 
@@ -340,6 +343,24 @@ def test_attention_of_sharp_scores_and_of_extreme_queries(dtype, n):
         out = c.attention(q2, start, ln, table, frame=1, max_new=n)
         err = (out[:ref.shape[0]].double().cpu() - ref).abs()
         assert not err.isnan().any() and ((err <= tol) | ~ok).all()
+
+
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
+def test_attention_scales(scale, n):
+    """0: the mean of what a row sees; below 0: the smallest product counts most."""
+    lens, heads, dim = [300, 41], 6, 96
+    c, q, start, ln, table, _, _ = attention_case(lens, [n, n], heads, 2, dim, 16, torch.float16, 1, 31)
+    out = c.attention(q, start, ln, table, scale=scale, frame=1, max_new=n)
+    t = table.cpu().tolist()
+    for r in range(2):
+        slots = torch.tensor([t[r][j // 16] * 16 + j % 16 for j in range(lens[r])], device="cuda")
+        k, v = (x.double().cpu() for x in c.load(slots, torch.float32))
+        for h in range(heads):
+            rows_ = slice(r * n, r * n + n)
+            o, mean, size = ref_attention(q[rows_, h].double().cpu(), k[:, h // 3], v[:, h // 3], torch.arange(lens[r] - n, lens[r]), 1, scale)
+            check(out[rows_, h], o, bound(o, mean, size, torch.float16))
+    c.check()                                             # no bounded wait ran out
 
 
 @pytest.mark.parametrize("size", [1e-6, 1.0, 3e4])
@@ -582,3 +603,15 @@ def test_refusals_on_the_device():
     assert b"slots is not memory of the current device" in L.jepa_error_text()
     L.jepa_error_reset()
     assert c.attention(q[:0], i32([0, 0]), ln, table).shape == (0, 4, 64)
+    # a workspace that is too small
+    a = kv4._Attn(q.data_ptr(), q.data_ptr(), 256, 64, 256, 64, start.data_ptr(), ln.data_ptr(), table.data_ptr(), 1, 3, 4000, 4, 1, 1,
+                  0.125, 0, 3, None, 0)
+    need = L.jepa_b200_kv4_attention_workspace(c._ref, kv4.C.byref(a))
+    a.workspace, a.workspace_bytes = q.data_ptr(), need - 1
+    assert need > 0 and L.jepa_b200_kv4_attention(c._ref, kv4.C.byref(a), None) == -1
+    assert b"the workspace holds" in L.jepa_error_text()
+    L.jepa_error_reset()
+    with pytest.raises(ValueError, match="2\\^30"):
+        kv4.build_tables(ln, ln, table, ln, 16, 2 ** 30 + 1)
+    with pytest.raises(ValueError, match="2\\^31"):
+        c.attention(q, start, ln, table, frame=2 ** 31)

@@ -80,7 +80,7 @@ def test_refused_rows():
 @pytest.mark.parametrize("bad,word", [
     (dict(type=0), "type 0"), (dict(n_heads=3), "query heads"), (dict(n_heads=0), "query heads"), (dict(n_heads=65536), "query heads"),
     (dict(n_req=-1), "requests"), (dict(n_req=65536), "requests"), (dict(n_rows=-1), "rows"), (dict(width=0), "columns"),
-    (dict(width=1 << 27), "2^31"), (dict(frame=-1), "frame"), (dict(max_len=-1), "max_len"), (dict(max_new=-2), "max_new"),
+    (dict(width=1 << 27), "2^31"), (dict(n_rows=(1 << 28) + 1), "2^30"), (dict(frame=-1), "frame"), (dict(max_len=-1), "max_len"), (dict(max_new=-2), "max_new"),
     (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(q_tok=-1), "strides"), (dict(o_tok=63), "overlap"),
     (dict(o_head=63), "overlap"), (dict(q=None), "q is null"), (dict(out=None), "out is null"), (dict(lens=PTR + 2), "lens must be 4-byte"),
     (dict(table=None), "table is null"), (dict(q_start=None), "q_start is null"), (dict(q=PTR + 1), "q must be 2-byte")])
@@ -102,7 +102,8 @@ def test_attention_over_nothing_is_no_call():
 
 
 @pytest.mark.parametrize("bad,word", [(dict(n_req=0), "n_req"), (dict(width=0), "width"), (dict(n_free=-1), "n_free"),
-                                      (dict(n_slots=0), "n_slots"), (dict(page=24), "page_size"), (dict(page=8), "page_size"),
+                                      (dict(n_slots=0), "n_slots"), (dict(n_slots=(1 << 30) + 1), "2^30"), (dict(n_req=(1 << 30) + 1), "2^30"),
+                                      (dict(n_free=(1 << 30) + 1), "2^30"), (dict(page=24), "page_size"), (dict(page=8), "page_size"),
                                       (dict(cached=None), "cached is null"), (dict(slots=PTR + 4), "slots must be 8-byte"),
                                       (dict(free=None), "free_pages is null"), (dict(state=PTR + 2), "state must be 4-byte")])
 def test_refused_tables(bad, word):
