@@ -232,10 +232,12 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
             read = read == (STAGES - 1) * SB ? 0 : read + SB;
             const __half * kd = (const __half *) (vb + STEP * RB), * vd = kd + NG * STEP;
             const int key = k0 + STEP * (WARPS * i + warp);
-            // ---- scores
-            float s[2][NT][4];
-#pragma unroll
+            // two tiles of 16 keys, one after the other (side by side in one body of twice the length, the schedulers waited for
+            // instructions: 121 us for 64 sessions of 1000 .. 8190 keys)
+#pragma unroll 1
             for (int u = 0; u < 2; u++) {
+                // ---- scores
+                float s[NT][4];
                 uint32_t w[2][NG];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
@@ -265,78 +267,66 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const float d = e < 2 ? d0 : d1;
-                            s[u][nt][e] = gi == 0 ? d * acc[e] : __fmaf_rn(d, acc[e], s[u][nt][e]);
+                            s[nt][e] = gi == 0 ? d * acc[e] : __fmaf_rn(d, acc[e], s[nt][e]);
                         }
                     }
                 }
-            }
-            const bool whole = key + STEP <= min(low, k1) && hole == 0;
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) s[u][nt][e] *= sl2[nt][e & 1];
-                }
-            }
-            if (!whole) {
+                const bool whole = key + 16 * u + 16 <= min(low, k1) && !((hole >> u) & 1);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
+                    for (int e = 0; e < 4; e++) s[nt][e] *= sl2[nt][e & 1];
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const int k = key + 16 * u + 8 * (e >> 1) + g;
-                            if (k >= min(lim[nt][e & 1], k1) || ((hole >> u) & 1)) s[u][nt][e] = -INFINITY;
+                            if (k >= min(lim[nt][e & 1], k1) || ((hole >> u) & 1)) s[nt][e] = -INFINITY;
                         }
                     }
+                    asm volatile("" ::: "memory");               // a branch, not selects in every step
                 }
-                asm volatile("" ::: "memory");               // a branch, not selects in every step
-            }
-            float mx[NT][2];
-            bool raise = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    mx[nt][e] = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
-                    raise = raise || mx[nt][e] - z[nt][e] > 14.0f;
-                }
-            }
-            if (__any_sync(0xffffffffu, raise)) {
+                float mx[NT][2];
+                bool raise = false;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        float x = mx[nt][e];
-#pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                        x = fmaxf(below(x), z[nt][e]);
-                        const float c = x == z[nt][e] ? 1.0f : ex2(z[nt][e] - x);
-                        z[nt][e] = x;
-                        l[nt][e] *= c;
-#pragma unroll
-                        for (int k = 0; k < MT; k++) { o[k][nt][e] *= c; o[k][nt][e + 2] *= c; }
+                        mx[nt][e] = fmaxf(s[nt][e], s[nt][e + 2]);
+                        raise = raise || mx[nt][e] - z[nt][e] > 14.0f;
                     }
                 }
-            }
-            // ---- weights, as the B operand of the second product
-            uint32_t pf[2][NT][2];
+                if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
+                    for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const float p0 = ex2(s[u][nt][0] - z[nt][0]), p1 = ex2(s[u][nt][1] - z[nt][1]);
-                    const float p2 = ex2(s[u][nt][2] - z[nt][0]), p3 = ex2(s[u][nt][3] - z[nt][1]);
+                        for (int e = 0; e < 2; e++) {
+                            float x = mx[nt][e];
+#pragma unroll
+                            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                            x = fmaxf(below(x), z[nt][e]);
+                            const float c = x == z[nt][e] ? 1.0f : ex2(z[nt][e] - x);
+                            z[nt][e] = x;
+                            l[nt][e] *= c;
+#pragma unroll
+                            for (int k = 0; k < MT; k++) { o[k][nt][e] *= c; o[k][nt][e + 2] *= c; }
+                        }
+                    }
+                }
+                // ---- weights, as the B operand of the second product
+                uint32_t pf[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    const float p0 = ex2(s[nt][0] - z[nt][0]), p1 = ex2(s[nt][1] - z[nt][1]);
+                    const float p2 = ex2(s[nt][2] - z[nt][0]), p3 = ex2(s[nt][3] - z[nt][1]);
                     l[nt][0] += p0 + p2;
                     l[nt][1] += p1 + p3;
-                    pf[u][nt][0] = transpose8(pack_h2(p0, p1));
-                    pf[u][nt][1] = transpose8(pack_h2(p2, p3));
+                    pf[nt][0] = transpose8(pack_h2(p0, p1));
+                    pf[nt][1] = transpose8(pack_h2(p2, p3));
                 }
-            }
             // ---- sums of values
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
                 const int ra = 16 * u + 2 * t;                         // this lane's keys: ra, ra + 1, ra + 8, ra + 9
                 constexpr int PARTS = NG % 2 ? NG : NG / 2;           // 32 or 64 channels at a time
 #pragma unroll
@@ -381,8 +371,8 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
                         const int mt = NG % 2 ? 2 * j : 4 * j + 2 * h;
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
-                            mma16816(o[mt][nt], {h2u(x[0]), h2u(x[1]), h2u(y[0]), h2u(y[1])}, pf[u][nt][0], pf[u][nt][1]);
-                            mma16816(o[mt + 1][nt], {h2u(x[2]), h2u(x[3]), h2u(y[2]), h2u(y[3])}, pf[u][nt][0], pf[u][nt][1]);
+                            mma16816(o[mt][nt], {h2u(x[0]), h2u(x[1]), h2u(y[0]), h2u(y[1])}, pf[nt][0], pf[nt][1]);
+                            mma16816(o[mt + 1][nt], {h2u(x[2]), h2u(x[3]), h2u(y[2]), h2u(y[3])}, pf[nt][0], pf[nt][1]);
                         }
                     }
                 }

@@ -2,7 +2,7 @@
 //
 // One CTA per (request, cache head, 256 columns, range of keys); a column is a (new token, head of the group) pair, a
 // row of the two 128-row tiles here. Keys come in blocks of 64. Warps:
-//   0 .. 7   softmax: one thread per row (4 warps a tile, one per TMEM lane quadrant). They write the queries into TMEM
+//   0 .. 7   softmax: one thread per row (4 warps a tile, one per TMEM lane quadrant). They put the queries in place
 //            once (scaled by a power of two into f16's range), then per block read their row of S = Q K^T from
 //            TMEM once, and put the weights P = 2^(s - z) back in f16 over the front half of S's
 //            columns, where the second product takes it as its A operand: P never passes through shared memory.
@@ -11,13 +11,21 @@
 //   8 .. 11  conversion from 4 bits to d (c - 8) in f16 (exact, kv4.h), one thread per row: two warps for K, two for V,
 //            written in the 128-byte swizzle of the products' operands (K: K-major; V: MN-major, keys down
 //            the rows). The next block's codes are loaded before this one's are converted; four blocks are held.
-//   12, 13   issue the products of tile 0 and 1: S_t = Q_t K^T (M 128, N 64) and O_t += P_t V (M 128, N hd). Both take A from
-//            TMEM: the tensor core reads shared memory at about 64 bytes a cycle, so that with Q there too a 128 x 64 x 16
-//            product took 100 cycles instead of 32. Up to head_dim 64 TMEM has room for two buffers of S a tile, and
-//            the scores run two blocks ahead; above that the tiles' turns hide each other's products.
+//   12, 13   issue the products of tile 0 and 1: S_t = Q_t K^T (M 128, N 64), two blocks ahead in two buffers, and
+//            O_t += P_t V (M 128, N hd). Softmax never waits for a product of its own block, and the tiles run on
+//            their own.
+// Up to head_dim 64 TMEM holds Q beside S and O, above that Q stays in shared memory. The tensor core reads shared memory, and A
+// in TMEM, at about 64 bytes a cycle each: a 128 x 64 x 16 product takes 64 cycles with Q in TMEM and 100 with Q in shared
+// memory, 128 x 128 x 16 (P V at head_dim 128) 64. What bounds it: at head_dim 128 the products, 2100 of the 2700 cycles a pair
+// of tiles takes for 64 keys (chunks of 700 .. 2047 rows behind 4100 .. 8191 keys, 32 / 8 heads: 730 us, 673 TFLOP/s); at
+// head_dim 64 the softmax, 1024 of 2300 cycles of which are exponentials (96 x 258 rows over 774 keys, 16 heads: 250 us
+// of 299, the rest is the rows kernel's for the last 2 rows).
+// Measured and not taken, at head_dim 128: 128 keys a block with one buffer of S, 784 us or more (the softmax waits 2200 cycles
+// a block); Q in TMEM with one buffer, 858; two blocks' scores in one product of N 128, 884; turns of the two tiles' exponentials,
+// 756 against 742; a quarter of the exponentials as polynomials, no change (head_dim 64: 301 instead of 312).
 // Within 8 channels the operands keep the order in which codes unpack, 0 4 1 5 2 6 3 7: Q is written in the order of
 // K's words, O's columns are put right when they are stored.
-// TMEM columns: O_0, O_1 (hd each), Q_0, Q_1 (hd / 2), then the buffers of S.
+// TMEM columns: O_0, O_1 (hd each), Q_0, Q_1 (hd / 2) up to head_dim 64, then two buffers of S a tile.
 // A value scale that is not finite enters as zeros; the rows that see such a key get NaN in that group at the end, so a NaN
 // behind a row's mask does not reach it (0 * NaN).
 // Every mbarrier wait is bounded: on a timeout the kernel raises the error flag, its rows become NaN, and it ends.
