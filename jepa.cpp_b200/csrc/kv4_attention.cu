@@ -62,6 +62,8 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
+__device__ __forceinline__ void wait_for_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 constexpr int STEP = 32;        // keys a warp takes at a time
 constexpr int STAGES = 2;          // (3: 128 us for 64 sessions of 1000 .. 8190 keys instead of 121)
 constexpr int WARPS = 4;
@@ -83,7 +85,10 @@ template <class T, int NG, int NT>
 __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const Kv4Pool pool, const Kv4Attn a, const Split sp, int tiles,
                                                                           int vec, int rest) {
     constexpr int HD = 32 * NG, RB = row_bytes<NG>(), SB = stage_bytes<NG>(), MT = 2 * NG;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // After the tiles kernel (rest) the wait comes last: this grid starts when all of that kernel's CTAs have passed their own
+    // wait, so what both read is there, and it runs on the SMs that its last CTAs leave idle; the wait at the
+    // end keeps whatever follows behind both.
+    if (!rest) wait_for_grid();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ uint32_t s_poison[8 * NT];
@@ -93,7 +98,10 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
     const Req rq = request_of(a, pool.page_shift, r);
     const int n_cols = (rq.row1 - rq.row0) * G;              // (token, head of the group) columns of this cache head
     const int span = sp.span(rq.len), used = sp.used(rq.len);
-    if (n_cols <= 0 || (blockIdx.x && (int) blockIdx.x >= used)) return;
+    if (n_cols <= 0 || (blockIdx.x && (int) blockIdx.x >= used)) {
+        if (rest) wait_for_grid();
+        return;
+    }
     const int k0 = blockIdx.x * span, k1 = range_end(rq.len, k0, span);
     const int32_t * table = a.table + (size_t) r * a.width;
     const int n_pages = (int) (pool.n_slots >> pool.page_shift), pmask = (1 << pool.page_shift) - 1;
@@ -439,6 +447,7 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
         }
         __syncthreads();
     }
+    if (rest) wait_for_grid();
 }
 
 // Joins the partial sums of a row: one CTA per (row, head), its warps taking every eighth part.
