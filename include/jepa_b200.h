@@ -228,8 +228,8 @@ int64_t jepa_b200_kv4_attention_workspace(const jepa_b200_kv4_cache * cache, con
 int jepa_b200_kv4_attention(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, void * stream);
 
 // Waits for `stream` and reports (and clears) the failure flag of the attention's bounded device waits on the current
-// device: 0, or -1 with the reason when a kernel gave up on its pipeline (its rows are NaN then). Not for a capturing
-// stream.
+// device: 0, or -1 with the reason when a kernel gave up on its pipeline (its rows are NaN then). A capturing stream is
+// refused.
 int jepa_b200_kv4_check(void * stream);
 
 #if defined(__GNUC__)

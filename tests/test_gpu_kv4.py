@@ -540,6 +540,33 @@ def test_steps_of_growing_sessions(captured):
     assert used == sum(-(-x.shape[0] // page) for x in s.k)
 
 
+def test_a_captured_chunk_follows_its_inputs():
+    """Tiles, left-over columns, key ranges and their merge in one graph, replayed for other lengths and row counts than
+    it was captured with; the check of the waits refuses to be captured and leaves the capture as it was."""
+    new, lens = [100, 3, 258], [1500, 900, 2500]
+    c, q, start, ln, table, ref, tol = attention_case(lens, new, 2, 2, 64, 32, torch.float16, 258, 17)
+    out = torch.zeros_like(q)
+    some_start, some_len = i32([0, 1, 2, 3]), i32([5, 6, 7])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c.attention(q, some_start, some_len, table, frame=258, max_len=2500, max_new=258, out=out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        c.attention(q, some_start, some_len, table, frame=258, max_len=2500, max_new=258, out=out)
+        with pytest.raises(RuntimeError, match="capturing"):
+            c.check()
+    some_start.copy_(start)
+    some_len.copy_(ln)
+    for _ in range(3):
+        out.fill_(5.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out, ref, tol)
+        assert (out[ref.shape[0]:] == 5.0).all()
+    c.check()
+
+
 def test_two_graphs_and_a_third_stream_at_once():
     """Graphs captured one after the other do not share what a call leaves behind: replayed side by side they agree
     with the eager calls."""
