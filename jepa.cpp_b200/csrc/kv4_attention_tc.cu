@@ -19,7 +19,7 @@
 // memory, 128 x 128 x 16 (P V at head_dim 128) 64. What bounds it: at head_dim 128 the products, 2100 of the 2700 cycles a pair
 // of tiles takes for 64 keys (chunks of 700 .. 2047 rows behind 4100 .. 8191 keys, 32 / 8 heads: 730 us, 673 TFLOP/s); at
 // head_dim 64 the softmax, 1024 of 2300 cycles of which are exponentials (96 x 258 rows over 774 keys, 16 heads: 250 us
-// of 299, the rest is the rows kernel's for the last 2 rows).
+// of 285, the rest is the rows kernel's for the last 2 rows).
 // Measured and not taken, at head_dim 128: 128 keys a block with one buffer of S, 784 us or more (the softmax waits 2200 cycles
 // a block); Q in TMEM with one buffer, 858; two blocks' scores in one product of N 128, 884; turns of the two tiles' exponentials,
 // 756 against 742; a quarter of the exponentials as polynomials, no change (head_dim 64: 301 instead of 312).

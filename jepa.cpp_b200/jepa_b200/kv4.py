@@ -111,16 +111,21 @@ def build_tables(cached: torch.Tensor, added: torch.Tensor, table: torch.Tensor,
     _index(added, "added", torch.int32, dev)
     _index(table, "table", torch.int32, dev, 2)
     _index(free_pages, "free_pages", torch.int32, dev)
-    _need(added.shape[0] == n and table.shape[0] == n, "cached, added and table must have one entry a request")
-    _need(n >= 1 and table.shape[1] >= 1, "there must be a request and a table column")
-    _need(max(n, table.shape[1], free_pages.shape[0], n_slots, page_size) <= 2 ** 30, "no count may pass 2^30")
+    rows, width = table.shape
+    n_free = free_pages.shape[0]
+    if added.shape[0] != n or rows != n:
+        raise ValueError("cached, added and table must have one entry a request")
+    if not (n >= 1 and width >= 1):
+        raise ValueError("there must be a request and a table column")
+    if not (1 <= n_slots <= 2 ** 30 and max(n, width, n_free, page_size) <= 2 ** 30):
+        raise ValueError("n_slots must be 1 or more, and no count may pass 2^30")
     # lens, q_start and state share one allocation, each at a multiple of 4 bytes
-    ints = torch.empty(2 * n + 3, dtype=torch.int32, device=dev)
-    lens, q_start, state = ints.split((n, n + 1, 2))
-    slots = torch.empty(n_slots, dtype=torch.int64, device=dev)
+    ints = cached.new_empty(2 * n + 3)
+    lens, q_start, state = torch.split_with_sizes(ints, (n, n + 1, 2))
+    slots = cached.new_empty(n_slots, dtype=torch.int64)
     base = ints.data_ptr()
-    _call("jepa_b200_kv_tables", dev, cached.data_ptr(), added.data_ptr(), n, page_size, table.data_ptr(), table.shape[1],
-          free_pages.data_ptr(), free_pages.shape[0], base, base + 4 * n, slots.data_ptr(), n_slots, base + 4 * (2 * n + 1))
+    _call("jepa_b200_kv_tables", dev, cached.data_ptr(), added.data_ptr(), n, page_size, table.data_ptr(), width,
+          free_pages.data_ptr(), n_free, base, base + 4 * n, slots.data_ptr(), n_slots, base + 4 * (2 * n + 1))
     return Tables(lens, q_start, slots, state)
 
 
@@ -184,11 +189,12 @@ class KV4Cache:
     def load(self, slots: torch.Tensor, dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
         """The values cached in slots [n] (int64): k, v [n, kv_heads, head_dim]; zeros for a slot outside the pool."""
         _index(slots, "slots", torch.int64, self._dev)
-        _need(dtype in _TYPE, f"{dtype} is not f32, f16 or bf16")
-        shape = (slots.shape[0], self.kv_heads, self.head_dim)
-        k = torch.empty(shape, dtype=dtype, device=self._dev)
-        v = torch.empty(shape, dtype=dtype, device=self._dev)
-        _call("jepa_b200_kv4_load", self._dev, self._ref, slots.data_ptr(), shape[0], k.data_ptr(), v.data_ptr(), _TYPE[dtype])
+        if dtype not in _TYPE:
+            raise ValueError(f"{dtype} is not f32, f16 or bf16")
+        n = slots.shape[0]
+        k = self.d.new_empty((n, self.kv_heads, self.head_dim), dtype=dtype)
+        v = torch.empty_like(k)
+        _call("jepa_b200_kv4_load", self._dev, self._ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), _TYPE[dtype])
         return k, v
 
     def attention(self, q: torch.Tensor, q_start: torch.Tensor, lens: torch.Tensor, table: torch.Tensor,
