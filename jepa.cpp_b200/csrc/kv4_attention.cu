@@ -505,9 +505,9 @@ struct Plan {
 Plan plan_of(const Kv4Pool & p, const Kv4Attn & a) {
     Plan r;
     const long long cols = (long long) a.max_new * (a.heads / p.heads);
-    r.tc = cols > 16;
+    r.tc = cols > FEW;
     r.nt = (r.tc ? cols % 256 : cols) > 8 ? 2 : 1;
-    if (r.tc) r.tiles = (int) std::min<long long>((cols + 255 - 16) / 256, 65535 / p.heads);
+    if (r.tc) r.tiles = (int) std::min<long long>((cols + 255 - FEW) / 256, 65535 / p.heads);
     else r.tiles = (int) std::min<long long>((cols + 8 * r.nt - 1) / (8 * r.nt), 65535 / p.heads);
     // Ranges of 1024 keys or more, 4 to each of the 148 SMs x 4 resident CTAs if every request is as long as the longest
     // (fewer leave SMs idle at the end where lengths differ, more pay for starts and partial sums; 64 sessions of
@@ -531,7 +531,7 @@ size_t partial_bytes(const Kv4Pool & p, const Kv4Attn & a, int n_split) {
 
 template <class T, int NG, int NT>
 int rows_launch(const Kv4Pool & p, const Kv4Attn & a, const Plan & r, int vec, cudaStream_t st) {
-    const int tiles = r.tc ? 1 : r.tiles;
+    const int tiles = !r.tc ? r.tiles : NT == 1 ? 1 : 2;      // beside the tiles kernel: the columns it leaves
     constexpr int smem = rows_smem<NG, NT>();
     if (allow_smem<k_kv4_rows<T, NG, NT>>(smem)) return -1;
     const dim3 grid((unsigned) r.sp.n_split, (unsigned) (p.heads * tiles), (unsigned) a.n_req);

@@ -61,9 +61,12 @@ __device__ __forceinline__ int visible(const Req & q, int row, int frame) {
 }
 
 // Columns of a request and cache head that the tiles kernel takes, of n in all: whole tiles of 256, and what is left over if
-// it is more than 16; the rows kernel takes the rest. (258 columns in two CTAs of the tiles kernel: the second, for 2 of
-// them, took as long as the first.)
-__host__ __device__ inline int tile_columns(int n) { return n % 256 > 16 ? n : n - n % 256; }
+// it is more than 32; the rows kernel takes the rest, 16 at a time. 32 sessions of 6000 .. 8000 keys, 4 cache heads, head_dim 64 / 128:
+// 24 columns take the rows kernel 90 / 137 us and the tiles kernel 135 / 197, 32 columns 101 / 150 and 141 / 204; a third
+// and fourth pass over the cache would cost more than the tiles kernel, whose time hardly depends on the columns. (258
+// columns in two CTAs of the tiles kernel: the second, for 2 of them, took as long as the first.)
+constexpr int FEW = 32;
+__host__ __device__ inline int tile_columns(int n) { return n % 256 > FEW ? n : n - n % 256; }
 
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
