@@ -120,7 +120,6 @@ __device__ __forceinline__ void quantise_row(const Vec8<T> (&in)[NG], uint32_t (
 template <class T, int NG>
 __global__ void __launch_bounds__(128) k_kv4_store(const Kv4Pool p, const Kv4Rows r, const int64_t * __restrict__ slots, long long n,
                                                    bool vec) {
-    constexpr int HD = 32 * NG;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31, t = lane & 3;
@@ -161,7 +160,6 @@ __global__ void __launch_bounds__(128) k_kv4_store(const Kv4Pool p, const Kv4Row
     for (int g = 0; g < NG; g++) {
         if (t == g) { kd[(size_t) g * P] = ks[g]; vd[(size_t) g * P] = vs[g]; }
     }
-    (void) HD;
 }
 
 template <class T> __device__ __forceinline__ T to_type(float x);
