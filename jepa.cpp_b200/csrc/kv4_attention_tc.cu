@@ -50,7 +50,8 @@ constexpr int SOFT = 8, CONV = 4, PROD = 2;     // warps of each kind
 constexpr int THREADS = 32 * (SOFT + CONV + PROD);
 constexpr uint32_t QATOM = 128 * 128, ATOM = BLK * 128;     // bytes of 128 and of BLK rows of 64 f16
 constexpr int SLOTS = 8;                        // blocks whose key masks are kept: those in shared memory, and two that
-                                                // have left it as operands but not yet as scores
+                                                // have left it as operands but not yet as scores (S of block j - STAGES is
+                                                // done: the weights of block j - STAGES - 2 are there, its masks are read)
 
 __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn_major) {      // kind::f16, f16 in, f32 out, M 128
     return (1u << 4) | ((uint32_t) (n >> 3) << 17) | ((uint32_t) (128 >> 4) << 24) | (b_mn_major ? 1u << 16 : 0u);
@@ -331,6 +332,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                     const uint32_t ph = (uint32_t) (j / STAGES - 1) & 1u;
                     uint64_t (&empty)[2][STAGES] = keys ? bars.k_empty : bars.v_empty;
                     if (j - STAGES < nb0) ok = warp_wait(&empty[0][s], ph, 41);
+                    // Where tile 0 has no block j - STAGES, tile 1 alone would set the pace, and this block's masks could take
+                    // the place of tile 0's last ones before its softmax has read them: wait for tile 0's last product.
+                    else if (keys && j - STAGES == nb0 && nb0 > 0) ok = warp_wait(&bars.o_done[0][(nb0 - 1) % NB], (uint32_t) ((nb0 - 1) / NB) & 1u, 40);
                     if (ok && n_tiles == 2) ok = warp_wait(&empty[1][s], ph, 42);
                     if (!ok) break;
                 }

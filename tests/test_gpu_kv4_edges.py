@@ -1,0 +1,80 @@
+"""The 4-bit cache's attention where tiles, masks and what lies in the cache meet: long frames with pages that are not
+there and scales that are not numbers, in every kernel and split."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_kv4 import attention_case, bound
+
+pytestmark = pytest.mark.gpu
+
+NAN = float("nan")
+
+
+def masked_case(lens, new, heads, kv_heads, dim, page, dtype, frame, seed, gone=(), broken=()):
+    """Like attention_case, with the pages of the (request, page index) pairs `gone` taken out of the table, and the value
+    scale of group 0 of the (request, key) pairs `broken` not a number. ref holds NaN where a row sees such a key."""
+    c, q, start, ln, table, _, _ = attention_case(lens, new, heads, kv_heads, dim, page, dtype, frame, seed)
+    t = table.cpu().tolist()
+    T = sum(new)
+    ref, tol = torch.zeros(T, heads, dim, dtype=torch.float64), torch.zeros(T, heads, dim, dtype=torch.float64)
+    at, group, scale = 0, heads // kv_heads, 1 / math.sqrt(dim)
+    for r, (L, n) in enumerate(zip(lens, new)):
+        slots = torch.tensor([t[r][j // page] * page + j % page for j in range(L)], dtype=torch.int64)
+        k, v = (x.double().cpu() for x in c.load(slots.cuda(), torch.float32))
+        held = torch.tensor([(r, j // page) not in gone for j in range(L)], dtype=torch.bool)
+        bad = torch.tensor([(r, j) in broken for j in range(L)], dtype=torch.bool)
+        pos = torch.arange(L - n, L)
+        lim = torch.full_like(pos, L)
+        if frame:
+            lim = torch.where(pos < 0, 0, (torch.div(pos, frame, rounding_mode="floor") + 1) * frame).clamp(max=L)
+        see = (torch.arange(L) < lim.unsqueeze(1)) & held
+        for h in range(heads if n else 0):
+            kk, vv, qq = k[:, h // group], v[:, h // group], q[at:at + n, h].double().cpu()
+            s = (qq @ kk.T * scale).masked_fill(~see, -math.inf)
+            m = s.amax(1, keepdim=True)
+            p = torch.where(see, torch.exp(s - torch.where(m == -math.inf, 0.0, m)), 0.0)
+            z = p.sum(1, keepdim=True)
+            p = p / torch.where(z == 0, 1.0, z)
+            size = (qq.abs() @ kk.abs().T * scale).masked_fill(~see, 0.0).amax(1, keepdim=True)
+            mean = p @ vv.abs() + 2.0 ** -20 * (see.double() @ vv.abs())
+            o = p @ vv
+            tol[at:at + n, h] = bound(o, mean, size, dtype)
+            o[(see & bad).any(1), :32] = NAN
+            ref[at:at + n, h] = o
+        at += n
+    for r, i in gone:
+        table[r, i] = -3 if (r + i) % 2 else c.n_pages + i
+    for r, j in broken:
+        c.d[t[r][j // page], 1, :, 0, j % page] = NAN
+    return c, q, start, ln, table, ref, tol
+
+
+def check_nan(out, ref, tol, what=""):
+    got = out[:ref.shape[0]].double().cpu()
+    assert torch.equal(got.isnan(), ref.isnan()), f"{what} NaN in {(got.isnan() != ref.isnan()).sum()} wrong places"
+    ok = ~ref.isnan()
+    err = (got - ref).abs()[ok]
+    assert (err <= tol[ok]).all(), f"{what} {(err / tol[ok].clamp(min=1e-30)).max().item():.3g} of the bound"
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, torch.float16), (128, torch.bfloat16), (32, torch.bfloat16), (96, torch.float16)])
+@pytest.mark.parametrize("frame,before", [(512, 1), (576, 1), (576, 2), (1024, 1), (1568, 1)])
+def test_frames_longer_than_a_tile_with_missing_pages_and_broken_scales(frame, before, dim, dtype):
+    """The second tile of 128 columns sees a whole frame more than the first, 8 to 25 blocks of 64 keys. Pages are missing
+    at the end of the frame before and along the later one, and a value scale of the later frame is not a number: the
+    masks of both tiles must stay apart."""
+    n, page = frame + 128, 32
+    L = frame * (before + 1)                       # rows 0 .. 127 lie in the frame before, the others in the last
+    ends = frame * before // page
+    gone = {(0, ends - 1), (0, ends - 3)} | {(0, i) for i in range(ends + 5, L // page, 3)}
+    broken = {(0, frame * before + 6 * 64 + 40)}
+    if any((0, j // page) in gone for _, j in broken):
+        gone -= {(0, j // page) for _, j in broken}
+    c, q, start, ln, table, ref, tol = masked_case([L], [n], 2, 2, dim, page, dtype, frame, frame + dim, gone, broken)
+    assert ref[128:, :, :32].isnan().all() and not ref[:128].isnan().any()
+    for _ in range(3):
+        check_nan(c.attention(q, start, ln, table, frame=frame, max_len=L, max_new=n), ref, tol)
+    check_nan(c.attention(q, start, ln, table, frame=frame), ref, tol, "no bounds")
+    c.check()
