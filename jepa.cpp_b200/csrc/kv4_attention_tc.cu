@@ -172,7 +172,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
     __shared__ uint32_t tmem_sh;
     __shared__ int abort_sh;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const int warp = __shfl_sync(0xffffffffu, (int) (threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // warp: uniform to the compiler
     const int kh = blockIdx.y / tiles, r = blockIdx.z, G = a.heads / pool.heads;
@@ -239,6 +238,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
             }
         }
         cta_sync();                             // TMEM is there, and free of the columns before
+        // (not earlier: launch.h; a CTA that left above releases them by its end)
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         const uint32_t tmem = tmem_sh;
         float f = 0.0f;                         // of this row's scores, in log2 units
         int lim = 0;                            // keys this row sees

@@ -2,6 +2,9 @@
 // previous kernel in the stream is still running; it must execute griddepcontrol.wait before it touches
 // memory the previous kernel writes or reads. Inside a captured CUDA graph this becomes a programmatic
 // edge, so a dependent kernel's launch latency and prologue overlap its predecessor's tail.
+// A kernel that takes tensor memory executes griddepcontrol.launch_dependents only behind a block barrier that follows
+// its tcgen05.alloc: a dependent may take its own before it waits, and a block whose alloc then waits for a dependent's
+// columns on the same SM, while the dependent waits for this grid, would never end.
 #pragma once
 
 #include <cuda_runtime.h>
