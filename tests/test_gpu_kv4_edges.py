@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_kv4 import attention_case, bound
+from test_gpu_kv4 import attention_case, bound, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +78,23 @@ def test_frames_longer_than_a_tile_with_missing_pages_and_broken_scales(frame, b
         check_nan(c.attention(q, start, ln, table, frame=frame, max_len=L, max_new=n), ref, tol)
     check_nan(c.attention(q, start, ln, table, frame=frame), ref, tol, "no bounds")
     c.check()
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_row_ranges_outside_of_q_are_cut(n):
+    """Whatever q_start holds, a request has rows of q or none: ranges that end before they start are empty, also where
+    their difference passes 32 bits, and the others are cut to q."""
+    c, q, start, ln, table, ref, tol = attention_case([300, 200], [n, n], 4, 2, 64, 32, torch.float16, 0, 5, tail=0)
+    low, high = -2 ** 31, 2 ** 31 - 1
+    for s in ([low, low, low], [n, low, n], [high, low, high], [high, high, high], [2 * n, low, high], [high, -1, low], [n, 0, low],
+              [low, n, low], [n, n, high], [-5, n, high]):
+        owner = torch.full((2 * n,), -1)
+        for r in range(2):
+            owner[min(max(0, s[r]), 2 * n):max(0, min(s[r + 1], 2 * n))] = r
+        own = owner == torch.arange(2 * n) // n                 # the rows that ref gives to their request
+        for bounds in (dict(max_len=300, max_new=n), {}):
+            out = torch.full_like(q, 7.0)
+            c.attention(q, i32(s), ln, table, out=out, **bounds)
+            got = out.double().cpu()
+            assert (got[owner < 0] == 7.0).all() and (got[owner >= 0] != 7.0).any(-1).all(), s
+            assert ((got - ref).abs() <= tol)[own].all(), s
