@@ -41,21 +41,20 @@ __device__ __forceinline__ int range_end(int len, int k0, int span) { return len
 // What a CTA needs to know of its request: rows [row0, row1) of q, keys [0, len) of the table. Whatever q_start holds,
 // 0 <= row0 <= row1 <= n_rows, so that row1 - row0 cannot overflow into a count of rows; a row that is there has last > row.
 struct Req {
-    int row0, row1, last, len, lens;
+    int row0, row1, last, len;
 };
 __device__ __forceinline__ Req request_of(const Kv4Attn & a, int page_shift, int r) {
     Req q;
     q.last = a.q_start[r + 1];
     q.row0 = min(max(0, a.q_start[r]), a.n_rows);
     q.row1 = max(q.row0, min(q.last, a.n_rows));
-    q.lens = a.lens[r];
-    q.len = (int) min((long long) max(q.lens, 0), (long long) a.width << page_shift);
+    q.len = (int) min((long long) max(a.lens[r], 0), (long long) a.width << page_shift);
     return q;
 }
 // keys that row `row` sees
 __device__ __forceinline__ int visible(const Req & q, int row, int frame) {
     if (frame == 0) return q.len;
-    const int p = q.lens - q.last + row;
+    const int p = q.len - q.last + row;
     if (p < 0) return 0;
     const long long lim = ((long long) p / frame + 1) * frame;
     return lim < q.len ? (int) lim : q.len;

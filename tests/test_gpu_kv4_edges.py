@@ -98,3 +98,20 @@ def test_row_ranges_outside_of_q_are_cut(n):
             got = out.double().cpu()
             assert (got[owner < 0] == 7.0).all() and (got[owner >= 0] != 7.0).any(-1).all(), s
             assert ((got - ref).abs() <= tol)[own].all(), s
+
+
+@pytest.mark.parametrize("n", [1, 5, 40, 300])
+@pytest.mark.parametrize("frame", [0, 1, 48])
+def test_lengths_past_the_table_are_cut_to_it(n, frame):
+    """lens is taken as at most width * page_size, for what is cached and for where the rows stand; below 0 it is 0."""
+    L, page = 208, 16                                   # 13 pages, each of them full: the table ends with the last key
+    c, q, start, ln, table, ref, tol = attention_case([L], [n], 4, 2, 64, page, torch.bfloat16, frame, 23, tail=1)
+    table = table[:, :L // page].contiguous()
+    for bounds in (dict(max_len=L, max_new=n), {}):
+        full = c.attention(q, start, ln, table, frame=frame, **bounds)
+        err = (full[:n].double().cpu() - ref).abs()
+        assert not full.isnan().any() and (err <= tol).all()
+        for length in (L + 1, 5 * L, 2 ** 31 - 1):
+            assert torch.equal(c.attention(q, start, i32([length]), table, frame=frame, **bounds), full), length
+        for length in (0, -1, -2 ** 31):
+            assert (c.attention(q, start, i32([length]), table, frame=frame, **bounds) == 0).all(), length
