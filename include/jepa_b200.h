@@ -225,6 +225,9 @@ typedef struct jepa_b200_kv4_attn {
     size_t workspace_bytes;   // it between calls, but calls that may run at once need one each
 } jepa_b200_kv4_attn;
 int64_t jepa_b200_kv4_attention_workspace(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args);
+// How that call is laid out, without making it: out[0] = 1 if many rows take the tiles kernel (0: all take the rows kernel),
+// out[1] = CTAs along a cache head's columns, out[2] = key ranges, out[3] = keys of a range. 0, or -1 for bad arguments.
+int jepa_b200_kv4_attention_plan(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, int * out);
 int jepa_b200_kv4_attention(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, void * stream);
 
 // Waits for `stream` and reports (and clears) the failure flag of the attention's bounded device waits on the current

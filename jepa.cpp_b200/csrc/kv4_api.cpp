@@ -161,6 +161,16 @@ int64_t jepa_b200_kv4_attention_workspace(const jepa_b200_kv4_cache * cache, con
     return (int64_t) jb::kv4_attention_workspace(p, a);
 }
 
+int jepa_b200_kv4_attention_plan(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, int * out) {
+    static const char * fn = "jepa_b200_kv4_attention_plan";
+    jb::Kv4Pool p;
+    jb::Kv4Attn a;
+    if (!pool_of(fn, cache, p) || !attn_of(fn, p, args, a)) return -1;
+    if (!out || !a.n_req || !a.n_rows) { log("jepa: %s: needs a result's pointer, requests and rows\n", fn); return -1; }
+    jb::kv4_attention_plan(p, a, out);
+    return 0;
+}
+
 int jepa_b200_kv4_attention(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, void * stream) {
     static const char * fn = "jepa_b200_kv4_attention";
     jb::Kv4Pool p;

@@ -496,7 +496,8 @@ __global__ void __launch_bounds__(256) k_kv4_merge(const Kv4Pool pool, const Kv4
     }
 }
 
-// The launch: which kernel, columns a CTA takes, CTAs along the columns, and the division of the keys.
+// The launch: which kernel, columns a CTA takes, CTAs along the columns, and the division of the keys. Counts of the whole
+// grid are taken in 64 bits: n_req, heads * tiles and max_len have 16, 16 and 31, and their product 63.
 struct Plan {
     bool tc;                    // the tiles kernel
     int nt, tiles;
@@ -504,22 +505,26 @@ struct Plan {
 };
 Plan plan_of(const Kv4Pool & p, const Kv4Attn & a) {
     Plan r;
-    const long long cols = (long long) a.max_new * (a.heads / p.heads);
+    const long long group = a.heads / p.heads, cols = a.max_new * group;
     r.tc = cols > FEW;
     r.nt = (r.tc ? cols % 256 : cols) > 8 ? 2 : 1;
     if (r.tc) r.tiles = (int) std::min<long long>((cols + 255 - FEW) / 256, 65535 / p.heads);
     else r.tiles = (int) std::min<long long>((cols + 8 * r.nt - 1) / (8 * r.nt), 65535 / p.heads);
+    // CTAs along requests and columns; where the rows of a request are not known, all requests together have n_rows
+    long long ctas = (long long) a.n_req * r.tiles;
+    if (a.max_new >= a.n_rows) ctas = std::min(ctas, a.n_req + a.n_rows * group / (r.tc ? 256 : 8 * r.nt));
     // Ranges of 1024 keys or more, 4 to each of the 148 SMs x 4 resident CTAs if every request is as long as the longest
     // (fewer leave SMs idle at the end where lengths differ, more pay for starts and partial sums; 64 sessions of
     // 1000 .. 8190 keys: 768 / 1536 / 2048 / 4096 keys a range = 121 / 115 / 116 / 126 us); down to 256 keys when a range
     // for each CTA is shorter than that.
-    const long long total = (long long) a.n_req * p.heads * r.tiles * a.max_len, slots = r.tc ? 148 : 148 * 4;
-    const long long chunk = std::max(std::max(256LL, std::min(1024LL, total / slots)), total / (4 * slots));
-    r.sp.chunk = (int) std::min<long long>((chunk + 127) & ~127LL, 0x7fffff00);
+    const long long total = ctas * p.heads * a.max_len, slots = r.tc ? 148 : 148 * 4;
+    const long long whole = (a.max_len + 127LL) & ~127LL;
+    long long chunk = (std::max(std::max(256LL, std::min(1024LL, total / slots)), total / (4 * slots)) + 127) & ~127LL;
     // one range where a second would be short or small: it would cost a second kernel (516 keys of one session: 8 us, against
     // 8 us in three ranges and 5 us of merge)
-    if (a.max_len <= 768 || a.max_len <= r.sp.chunk + r.sp.chunk / 4) r.sp.chunk = (a.max_len + 127) & ~127;
-    r.sp.n_split = (a.max_len + r.sp.chunk - 1) / r.sp.chunk;
+    if (a.max_len <= 768 || a.max_len <= chunk + chunk / 4) chunk = whole;
+    r.sp.chunk = (int) chunk;                                // at most `whole`, which is below 2^31 (attn_of)
+    r.sp.n_split = (int) ((a.max_len + chunk - 1) / chunk);
     r.sp.o = nullptr;
     r.sp.ml = nullptr;
     return r;
@@ -575,6 +580,14 @@ int launch_dim(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st) {
 size_t kv4_attention_workspace(const Kv4Pool & p, const Kv4Attn & a) {
     if (!a.n_req || !a.n_rows) return 0;
     return partial_bytes(p, a, plan_of(p, a).sp.n_split);
+}
+
+void kv4_attention_plan(const Kv4Pool & p, const Kv4Attn & a, int * out) {
+    const Plan r = plan_of(p, a);
+    out[0] = r.tc;
+    out[1] = r.tiles;
+    out[2] = r.sp.n_split;
+    out[3] = r.sp.chunk;
 }
 
 int kv4_attention(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st) {

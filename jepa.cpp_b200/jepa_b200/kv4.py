@@ -47,6 +47,7 @@ def _load() -> C.CDLL:
             "jepa_b200_kv4_store": (i32, [cp, vp, vp, C.c_uint32, i64, i64, i64, i64, vp, i64, vp]),
             "jepa_b200_kv4_load": (i32, [cp, vp, i64, vp, vp, C.c_uint32, vp]),
             "jepa_b200_kv4_attention_workspace": (i64, [cp, C.POINTER(_Attn)]),
+            "jepa_b200_kv4_attention_plan": (i32, [cp, C.POINTER(_Attn), C.POINTER(C.c_int)]),
             "jepa_b200_kv4_attention": (i32, [cp, C.POINTER(_Attn), vp]),
             "jepa_b200_kv4_check": (i32, [vp]),
         }

@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from test_gpu_kv4 import attention_case, bound, i32
+from jepa_b200 import kv4
+from test_gpu_kv4 import attention_case, bound, check, i32, ref_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -115,3 +116,29 @@ def test_lengths_past_the_table_are_cut_to_it(n, frame):
             assert torch.equal(c.attention(q, start, i32([length]), table, frame=frame, **bounds), full), length
         for length in (0, -1, -2 ** 31):
             assert (c.attention(q, start, i32([length]), table, frame=frame, **bounds) == 0).all(), length
+
+
+def test_many_requests_over_wide_tables_with_unknown_bounds():
+    """1024 requests of 64 rows whose tables could hold 4 million positions each, and no bounds: the launch is laid out for
+    what it is told, and the results are those of a call that knows better."""
+    R, n, dim, page, width = 1024, 64, 32, 256, 16384
+    g = torch.Generator("cuda").manual_seed(3)
+    c = kv4.KV4Cache(4, page, 1, dim)
+    x = torch.randn(2, 1024, 1, dim, generator=g, device="cuda")
+    c.store(x[0], x[1], torch.arange(1024, device="cuda"))
+    table = torch.full((R, width), -1, dtype=torch.int32, device="cuda")
+    table[:, 0], table[:, 1] = torch.arange(R, device="cuda") % 4, torch.arange(R, device="cuda") // 4 % 4
+    lens = (torch.arange(R, device="cuda", dtype=torch.int32) * 37) % 513
+    start = torch.arange(R + 1, device="cuda", dtype=torch.int32) * n
+    q = torch.randn(R * n, 1, dim, generator=g, device="cuda").half()
+    a = c.attention(q, start, lens, table, frame=1)
+    b = c.attention(q, start, lens, table, frame=1, max_len=512, max_new=n)
+    k, v = (t[:, 0].double().cpu() for t in c.load(torch.arange(1024, device="cuda"), torch.float32))
+    for r in (0, 1, 5, 500, 1023):
+        L = int(lens[r])
+        at = torch.tensor([int(table[r, j // page]) * page + j % page for j in range(L)], dtype=torch.int64)
+        o, mean, size = ref_attention(q[r * n:(r + 1) * n, 0].double().cpu(), k[at], v[at], torch.arange(L - n, L), 1, dim ** -0.5)
+        for out in (a, b):
+            check(out[r * n:(r + 1) * n, 0], o, bound(o, mean, size, torch.float16), f"request {r}")
+    half = torch.finfo(torch.float16).eps / 2
+    assert ((a - b).abs().double() <= 2 * half * b.abs().double() + 2 * 2.0 ** -11 * float(v.abs().max())).all()
