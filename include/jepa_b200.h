@@ -235,6 +235,12 @@ int jepa_b200_kv4_attention(const jepa_b200_kv4_cache * cache, const jepa_b200_k
 // refused.
 int jepa_b200_kv4_check(void * stream);
 
+// The same call with a failure made on purpose, for tests of what follows one: the kernel for many rows gives up at once
+// at its wait `wait` (40 .. 51, the number that jepa_b200_kv4_check names), and at the others, which may then never be
+// met, after limit_cycles (1 .. 4e9) clock cycles.
+int jepa_b200_kv4_attention_giving_up(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, int wait, long long limit_cycles,
+                                      void * stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

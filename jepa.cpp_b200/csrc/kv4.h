@@ -70,6 +70,8 @@ struct Kv4Attn {
     int type;
     void * ws;
     size_t ws_bytes;
+    long long wait_limit = 4000000000LL;    // cycles before a wait of the tiles kernel gives up (about 2 s)
+    int give_up_at = 0;                     // the wait (by its code) that gives up at once: the failure path's test
 };
 size_t kv4_attention_workspace(const Kv4Pool & p, const Kv4Attn & a);
 void kv4_attention_plan(const Kv4Pool & p, const Kv4Attn & a, int * out);      // see jepa_b200_kv4_attention_plan

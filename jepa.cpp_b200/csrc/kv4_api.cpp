@@ -93,6 +93,22 @@ bool row_type(const char * fn, uint32_t type) {
     return false;
 }
 
+// `a` comes with the limits of its waits
+int attention(const char * fn, const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, jb::Kv4Attn a, void * stream) {
+    jb::Kv4Pool p;
+    if (!pool_of(fn, cache, p) || !attn_of(fn, p, args, a)) return -1;
+    if (!a.n_req || !a.n_rows) return 0;
+    const size_t need = jb::kv4_attention_workspace(p, a);
+    if (a.ws_bytes < need) {
+        log("jepa: %s: the workspace holds %zu bytes, this call needs %zu\n", fn, a.ws_bytes, need);
+        return -1;
+    }
+    const void * ws = need ? a.ws : p.q;
+    if (device_pointers(fn, {{"cache.q", p.q, 16}, {"cache.d", p.d, 16}, {"q", a.q, 2}, {"out", a.out, 2}, {"q_start", a.q_start, 4},
+                             {"lens", a.lens, 4}, {"table", a.table, 4}, {"workspace", ws, 16}})) return -1;
+    return jb::kv4_attention(p, a, (cudaStream_t) stream);
+}
+
 }  // namespace
 
 extern "C" {
@@ -172,20 +188,20 @@ int jepa_b200_kv4_attention_plan(const jepa_b200_kv4_cache * cache, const jepa_b
 }
 
 int jepa_b200_kv4_attention(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, void * stream) {
-    static const char * fn = "jepa_b200_kv4_attention";
-    jb::Kv4Pool p;
-    jb::Kv4Attn a;
-    if (!pool_of(fn, cache, p) || !attn_of(fn, p, args, a)) return -1;
-    if (!a.n_req || !a.n_rows) return 0;
-    const size_t need = jb::kv4_attention_workspace(p, a);
-    if (a.ws_bytes < need) {
-        log("jepa: %s: the workspace holds %zu bytes, this call needs %zu\n", fn, a.ws_bytes, need);
+    return attention("jepa_b200_kv4_attention", cache, args, jb::Kv4Attn(), stream);
+}
+
+int jepa_b200_kv4_attention_giving_up(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, int wait, long long limit_cycles,
+                                      void * stream) {
+    static const char * fn = "jepa_b200_kv4_attention_giving_up";
+    if (wait < 40 || wait > 51 || limit_cycles < 1 || limit_cycles > 4000000000LL) {
+        log("jepa: %s: need 40 <= wait <= 51 and 1 <= limit_cycles <= 4e9 (%d, %lld)\n", fn, wait, limit_cycles);
         return -1;
     }
-    const void * ws = need ? a.ws : p.q;
-    if (device_pointers(fn, {{"cache.q", p.q, 16}, {"cache.d", p.d, 16}, {"q", a.q, 2}, {"out", a.out, 2}, {"q_start", a.q_start, 4},
-                             {"lens", a.lens, 4}, {"table", a.table, 4}, {"workspace", ws, 16}})) return -1;
-    return jb::kv4_attention(p, a, (cudaStream_t) stream);
+    jb::Kv4Attn a;
+    a.wait_limit = limit_cycles;
+    a.give_up_at = wait;
+    return attention(fn, cache, args, a, stream);
 }
 
 int jepa_b200_kv4_check(void * stream) {

@@ -28,7 +28,8 @@
 // TMEM columns: O_0, O_1 (hd each), Q_0, Q_1 (hd / 2) up to head_dim 64, then two buffers of S a tile.
 // A value scale that is not finite enters as zeros; the rows that see such a key get NaN in that group at the end, so a NaN
 // behind a row's mask does not reach it (0 * NaN).
-// Every mbarrier wait is bounded: on a timeout the kernel raises the error flag, its rows become NaN, and it ends.
+// Every mbarrier wait is bounded: when one runs out the CTA raises the error flag, waits for the products that it has issued,
+// writes NaN to the rows that it has not finished, and ends.
 #include "kv4_device.h"
 #include "common.h"
 #include "launch.h"
@@ -141,8 +142,12 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // the whole warp waits, and agrees on the outcome
-__device__ __forceinline__ bool warp_wait(uint64_t * bar, uint32_t parity, int code) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, code, &g_kv4_error));
+__device__ __forceinline__ bool warp_wait(const Kv4Attn & a, uint64_t * bar, uint32_t parity, int code) {
+    if (code == a.give_up_at) {
+        atomicExch(&g_kv4_error, code);
+        return false;
+    }
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, code, &g_kv4_error, a.wait_limit));
 }
 
 // bits of an f16 infinity or NaN
@@ -165,6 +170,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
     const uint32_t sQ = (smem_u32(smem_raw) + 1023) & ~1023u, sK = sQ + (QT ? 0 : 2 * AT * QATOM), sV = sK + STAGES * AT * ATOM;
     struct Bars {
         uint64_t k_full[STAGES], v_full[STAGES], k_empty[2][STAGES], v_empty[2][STAGES], s_full[2][NB], p_full[2][NB], o_done[2][NB];   // [tile][stage or buffer]
+        uint64_t drained[2];
     };
     __shared__ __align__(8) Bars bars;
     // per block and 32 keys: any exception; keys without a page; keys whose value scale of a group is not finite
@@ -187,7 +193,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
     }
     if (threadIdx.x == 0) abort_sh = 0;
 
-    for (int c0 = (int) (blockIdx.y % tiles) * 256; c0 < n_cols; c0 += tiles * 256) {
+    int c0 = (int) (blockIdx.y % tiles) * 256;
+    for (; c0 < n_cols; c0 += tiles * 256) {
         const int cols = min(256, n_cols - c0), n_tiles = cols > 128 ? 2 : 1;
         const int kend = min(visible(rq, rq.row0 + (c0 + cols - 1) / G, a.frame), k1);   // the last row sees most
         const int nb_all = kend > k0 ? (kend - k0 + BLK - 1) / BLK : 0;
@@ -200,6 +207,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                 for (int t = 0; t < 2; t++) { mbar_init(&bars.k_empty[t][s], 1); mbar_init(&bars.v_empty[t][s], 1); }
             }
             for (int t = 0; t < 2; t++) {
+                mbar_init(&bars.drained[t], 1);
                 // (one a buffer: a warp may be as many blocks ahead of another)
                 for (int i = 0; i < NB; i++) {
                     mbar_init(&bars.s_full[t][i], 1);
@@ -332,11 +340,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                 if (j >= STAGES) {
                     const uint32_t ph = (uint32_t) (j / STAGES - 1) & 1u;
                     uint64_t (&empty)[2][STAGES] = keys ? bars.k_empty : bars.v_empty;
-                    if (j - STAGES < nb0) ok = warp_wait(&empty[0][s], ph, 41);
+                    if (j - STAGES < nb0) ok = warp_wait(a, &empty[0][s], ph, 41);
                     // Where tile 0 has no block j - STAGES, tile 1 alone would set the pace, and this block's masks could take
                     // the place of tile 0's last ones before its softmax has read them: wait for tile 0's last product.
-                    else if (keys && j - STAGES == nb0 && nb0 > 0) ok = warp_wait(&bars.o_done[0][(nb0 - 1) % NB], (uint32_t) ((nb0 - 1) / NB) & 1u, 40);
-                    if (ok && n_tiles == 2) ok = warp_wait(&empty[1][s], ph, 42);
+                    else if (keys && j - STAGES == nb0 && nb0 > 0) ok = warp_wait(a, &bars.o_done[0][(nb0 - 1) % NB], (uint32_t) ((nb0 - 1) / NB) & 1u, 40);
+                    if (ok && n_tiles == 2) ok = warp_wait(a, &empty[1][s], ph, 42);
                     if (!ok) break;
                 }
                 if (keys) {
@@ -379,7 +387,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
             const uint32_t od = tmem + HD * t, qd = tmem + Q_COL + HD / 2 * t, sd = tmem + S_COL + NB * BLK * t;
             auto scores_of = [&](int j) -> bool {
                 const int s = j % STAGES;
-                if (!warp_wait(&bars.k_full[s], (uint32_t) (j / STAGES) & 1u, 43)) return false;
+                if (!warp_wait(a, &bars.k_full[s], (uint32_t) (j / STAGES) & 1u, 43)) return false;
                 fence_after();
                 const uint32_t id = idesc((min(BLK, kend - k0 - j * BLK) + 15) & ~15, false), ds = sd + BLK * (j % NB);
                 const uint32_t k_lo = k_desc + s * (AT * ATOM >> 4);
@@ -400,7 +408,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
             for (int j = 0; j < NB && j < nb && ok; j++) ok = scores_of(j);
             for (int j = 0; j < nb && ok; j++) {
                 const int s = j % STAGES;
-                ok = warp_wait(&bars.p_full[t][j % NB], (uint32_t) (j / NB) & 1u, 44) && warp_wait(&bars.v_full[s], (uint32_t) (j / STAGES) & 1u, 45);
+                ok = warp_wait(a, &bars.p_full[t][j % NB], (uint32_t) (j / NB) & 1u, 44) && warp_wait(a, &bars.v_full[s], (uint32_t) (j / STAGES) & 1u, 45);
                 if (!ok) break;
                 fence_after();
                 const int steps = (min(BLK, kend - k0 - j * BLK) + 15) / 16;
@@ -416,14 +424,21 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                 }
                 __syncwarp();
                 // the buffer's next scores go over P_t(j): only when its product is done
-                if (j + NB < nb) ok = warp_wait(&bars.o_done[t][j % NB], (uint32_t) (j / NB) & 1u, 46) && scores_of(j + NB);
+                if (j + NB < nb) ok = warp_wait(a, &bars.o_done[t][j % NB], (uint32_t) (j / NB) & 1u, 46) && scores_of(j + NB);
             }
             // the last arrivals of the commits, so that none meets a barrier that is set up anew
             for (int s = 0; s < STAGES && ok; s++) {
                 const int n = (nb + STAGES - 1 - s) / STAGES;
-                if (n > 0) ok = warp_wait(&bars.k_empty[t][s], (uint32_t) (n - 1) & 1u, 50) && warp_wait(&bars.v_empty[t][s], (uint32_t) (n - 1) & 1u, 51);
+                if (n > 0) ok = warp_wait(a, &bars.k_empty[t][s], (uint32_t) (n - 1) & 1u, 50) && warp_wait(a, &bars.v_empty[t][s], (uint32_t) (n - 1) & 1u, 51);
             }
-            if (!ok) abort_sh = 1;
+            if (!ok) {
+                // the products under way read shared memory and write tensor memory, both about to be given up
+                abort_sh = 1;
+                if (elect_one()) mma_commit(&bars.drained[t]);
+                __syncwarp();
+                mbar_wait(&bars.drained[t], 0, 52, &g_kv4_error);
+                __syncwarp();
+            }
         } else if (128 * (warp >> 2) + 32 * (warp & 3) < cols) {
             // ---- softmax: thread = row
             cta_sync();
@@ -434,7 +449,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
             uint32_t poison = 0;
             bool ok = true, plain = false;
             // O_t += P_t V of block j is done (a warp that asks has seen S(j) or S(j + 1), so block j - NB's is)
-            auto product_done = [&](int j, int code) -> bool { return warp_wait(&bars.o_done[t][j % NB], (uint32_t) (j / NB) & 1u, code); };
+            auto product_done = [&](int j, int code) -> bool { return warp_wait(a, &bars.o_done[t][j % NB], (uint32_t) (j / NB) & 1u, code); };
             // Raises z of the rows whose largest s - z of a block is `top` > 14.5 (z is a whole number, and so is the step:
             // sums and O take an exact power of two); returns the step.
             auto raise = [&](float top, int j) -> float {
@@ -443,8 +458,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                 const float down = ex2(-n);
                 z += n;
                 l *= down;
-                if (j > 0) {                    // O holds the blocks before this one
-                    ok = product_done(j - 1, 48);
+                if (j > 0) ok = product_done(j - 1, 48);
+                if (j > 0 && ok) {              // O holds the blocks before this one
                     fence_after();
 #pragma unroll 1
                     for (int i = 0; i < 2 * NG; i++) {
@@ -460,7 +475,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
             for (int j = 0; j < nb && ok; j++) {
                 const int key = k0 + j * BLK;
                 const uint32_t tb = ts + BLK * (j % NB);
-                if (!warp_wait(&bars.s_full[t][j % NB], (uint32_t) (j / NB) & 1u, 47)) { ok = false; break; }
+                if (!warp_wait(a, &bars.s_full[t][j % NB], (uint32_t) (j / NB) & 1u, 47)) { ok = false; break; }
                 fence_after();
                 uint32_t x[2][32];
                 tmem_ld32_async(tb, x[0]);
@@ -616,7 +631,19 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
             cta_sync();                         // a softmax warp without rows
         }
         cta_sync();
-        if (*(volatile int *) &abort_sh) break;
+        if (*(volatile int *) &abort_sh) {
+            // the columns that this CTA would have come to: not numbers either
+            for (c0 += tiles * 256; c0 < n_cols; c0 += tiles * 256) {
+                for (int i = threadIdx.x; i < min(256, n_cols - c0) * HD; i += THREADS) {
+                    const int col = c0 + i / HD, row = rq.row0 + col / G, head = kh * G + col % G;
+                    const size_t at = ((size_t) blockIdx.x * a.n_rows + row) * a.heads + head;
+                    if (used <= 1) ((T *) a.out)[(long long) row * a.o_tok + head * a.o_head + i % HD] = to_type<T>(__int_as_float(0x7fffffff));
+                    else sp.o[at * HD + i % HD] = __int_as_float(0x7fffffff);
+                    if (used > 1 && i % HD == 0) sp.ml[at] = make_float2(-FLT_MAX, 0.0f);
+                }
+            }
+            break;
+        }
         if (threadIdx.x == 0) {                 // the next columns start with fresh barriers
             for (int i = 0; i < (int) (sizeof(Bars) / 8); i++) {
                 asm volatile("mbarrier.inval.shared::cta.b64 [%0];" :: "r"(smem_u32((uint64_t *) &bars + i)) : "memory");

@@ -49,6 +49,7 @@ def _load() -> C.CDLL:
             "jepa_b200_kv4_attention_workspace": (i64, [cp, C.POINTER(_Attn)]),
             "jepa_b200_kv4_attention_plan": (i32, [cp, C.POINTER(_Attn), C.POINTER(C.c_int)]),
             "jepa_b200_kv4_attention": (i32, [cp, C.POINTER(_Attn), vp]),
+            "jepa_b200_kv4_attention_giving_up": (i32, [cp, C.POINTER(_Attn), i32, C.c_longlong, vp]),
             "jepa_b200_kv4_check": (i32, [vp]),
         }
         for name, (res, args) in sig.items():
