@@ -230,9 +230,10 @@ int64_t jepa_b200_kv4_attention_workspace(const jepa_b200_kv4_cache * cache, con
 int jepa_b200_kv4_attention_plan(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, int * out);
 int jepa_b200_kv4_attention(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, void * stream);
 
-// Waits for `stream` and reports (and clears) the failure flag of the attention's bounded device waits on the current
-// device: 0, or -1 with the reason when a kernel gave up on its pipeline (its rows are NaN then). A capturing stream is
-// refused.
+// Waits for `stream`, then reports the attention kernels of the current device, on whatever stream, that have given up one
+// of their bounded waits since the last report: 0, or -1 with the reason (their unfinished rows are NaN). A failure is
+// reported once, to whichever call comes first, so a program of several streams checks in one place, behind all of
+// them. A capturing stream is refused.
 int jepa_b200_kv4_check(void * stream);
 
 // The same call with a failure made on purpose, for tests of what follows one: the kernel for many rows gives up at once

@@ -76,6 +76,7 @@ struct Kv4Attn {
 size_t kv4_attention_workspace(const Kv4Pool & p, const Kv4Attn & a);
 void kv4_attention_plan(const Kv4Pool & p, const Kv4Attn & a, int * out);      // see jepa_b200_kv4_attention_plan
 int kv4_attention(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st);
-int kv4_error_flag(cudaStream_t st);            // waits for the stream; reads and resets: 0, or the wait that ran out (-1: not read)
+// Waits for the stream: the wait that ran out in a kernel of the current device, if one did that no call has told yet; 0, or -1: not read
+int kv4_error_flag(cudaStream_t st);
 
 }  // namespace jb

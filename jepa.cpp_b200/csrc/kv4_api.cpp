@@ -209,7 +209,7 @@ int jepa_b200_kv4_check(void * stream) {
     JB_CUDA(cudaStreamIsCapturing((cudaStream_t) stream, &capturing));
     if (capturing != cudaStreamCaptureStatusNone) { log("jepa: jepa_b200_kv4_check: the stream is capturing\n"); return -1; }
     const int code = jb::kv4_error_flag((cudaStream_t) stream);
-    if (code > 0) log("jepa: jepa_b200_kv4_check: an attention kernel gave up waiting on its pipeline (wait %d); its rows are NaN\n", code);
+    if (code > 0) log("jepa: jepa_b200_kv4_check: an attention kernel gave up waiting on its pipeline (wait %d); the rows that it had not finished are NaN\n", code);
     return code == 0 ? 0 : -1;
 }
 

@@ -35,11 +35,15 @@
 #include "launch.h"
 #include "tcgen05.cuh"
 
+#include <atomic>
 #include <cfloat>
 
 namespace jb {
 
-__device__ int g_kv4_error = 0;
+// The wait that ran out last, and how many CTAs have given up one. The device only counts; the host remembers how far it has told
+// (kv4_error_flag), so that what is raised while another thread or stream reads is told the next time.
+struct Kv4Failures { int code; unsigned count; };
+__device__ Kv4Failures g_kv4_failures = {0, 0};
 
 namespace {
 
@@ -144,10 +148,10 @@ __device__ __forceinline__ bool elect_one() {
 // the whole warp waits, and agrees on the outcome
 __device__ __forceinline__ bool warp_wait(const Kv4Attn & a, uint64_t * bar, uint32_t parity, int code) {
     if (code == a.give_up_at) {
-        atomicExch(&g_kv4_error, code);
+        atomicExch(&g_kv4_failures.code, code);
         return false;
     }
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, code, &g_kv4_error, a.wait_limit));
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, code, &g_kv4_failures.code, a.wait_limit));
 }
 
 // bits of an f16 infinity or NaN
@@ -436,7 +440,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
                 abort_sh = 1;
                 if (elect_one()) mma_commit(&bars.drained[t]);
                 __syncwarp();
-                mbar_wait(&bars.drained[t], 0, 52, &g_kv4_error);
+                mbar_wait(&bars.drained[t], 0, 52, &g_kv4_failures.code);
                 __syncwarp();
             }
         } else if (128 * (warp >> 2) + 32 * (warp & 3) < cols) {
@@ -632,6 +636,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
         }
         cta_sync();
         if (*(volatile int *) &abort_sh) {
+            if (threadIdx.x == 0) atomicAdd(&g_kv4_failures.count, 1u);
             // the columns that this CTA would have come to: not numbers either
             for (c0 += tiles * 256; c0 < n_cols; c0 += tiles * 256) {
                 for (int i = threadIdx.x; i < min(256, n_cols - c0) * HD; i += THREADS) {
@@ -677,14 +682,20 @@ int launch_dim(const Kv4Pool & p, const Kv4Attn & a, const Split & sp, int tiles
 }  // namespace
 
 int kv4_error_flag(cudaStream_t st) {
-    int v = 0;
-    static const int zero = 0;
-    if (!cuda_ok(cudaMemcpyFromSymbolAsync(&v, g_kv4_error, sizeof(int), 0, cudaMemcpyDeviceToHost, st), "reading the 4-bit cache's error flag") ||
-        !cuda_ok(cudaMemcpyToSymbolAsync(g_kv4_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st), "resetting the 4-bit cache's error flag") ||
-        !cuda_ok(cudaStreamSynchronize(st), "reading the 4-bit cache's error flag")) {
+    constexpr int DEVICES = 256;
+    static std::atomic<unsigned> told[DEVICES];
+    int dev = 0;
+    Kv4Failures v = {0, 0};
+    if (!cuda_ok(cudaGetDevice(&dev), "reading the 4-bit cache's failures") || dev >= DEVICES ||
+        !cuda_ok(cudaMemcpyFromSymbolAsync(&v, g_kv4_failures, sizeof(v), 0, cudaMemcpyDeviceToHost, st), "reading the 4-bit cache's failures") ||
+        !cuda_ok(cudaStreamSynchronize(st), "reading the 4-bit cache's failures")) {
         return -1;
     }
-    return v;
+    unsigned last = told[dev].load();
+    while ((int) (v.count - last) > 0) {                     // (another thread may have told a later count)
+        if (told[dev].compare_exchange_weak(last, v.count)) return v.code;
+    }
+    return 0;
 }
 
 int kv4_tiles(const Kv4Pool & p, const Kv4Attn & a, const Split & sp, int tiles, int vec, cudaStream_t st) {

@@ -241,5 +241,6 @@ class KV4Cache:
         return out
 
     def check(self) -> None:
-        """Waits for the current stream; raises if an attention kernel on it gave up waiting (its rows are NaN)."""
+        """Waits for the current stream; raises if an attention kernel of this device, on any stream, has given up a wait
+        that no check has told yet (the rows that it had not finished are NaN). Check in one place, behind all streams."""
         _call("jepa_b200_kv4_check", self._dev)

@@ -71,3 +71,51 @@ def test_a_wait_that_gives_up(wait, shape, dim, dtype):
         c.check()
     check(c.attention(q, start, ln, table, frame=frame, max_len=max_len, max_new=max_new), ref, tol)
     c.check()
+
+
+@pytest.mark.gpu
+def test_a_failure_is_told_once_whoever_asks():
+    from test_gpu_kv4 import attention_case
+    c, q, start, ln, table, _, _ = attention_case([300], [100], 1, 1, 64, 32, torch.float16, 1, 3)
+    out = torch.zeros_like(q)
+    side = torch.cuda.Stream()
+
+    def told(stream):
+        with torch.cuda.stream(stream):
+            try:
+                c.check()
+            except RuntimeError as e:
+                assert "gave up" in str(e)
+                return 1
+        return 0
+
+    here = torch.cuda.current_stream()
+    assert told(here) == 0
+    with torch.cuda.stream(side):
+        giving_up(c, q, start, ln, table, out, 43, 1, 300, 100)
+    assert (told(here), told(side), told(here)) == (1, 0, 0)
+    giving_up(c, q, start, ln, table, out, 47, 1, 300, 100)
+    giving_up(c, q, start, ln, table, out, 44, 1, 300, 100)
+    assert (told(side), told(here)) == (1, 0)
+
+
+@pytest.mark.gpu
+def test_a_failure_during_a_check_is_not_lost():
+    """Checks on one stream while kernels of another give up: one of those that follow a failure tells it."""
+    from test_gpu_kv4 import attention_case
+    c, q, start, ln, table, _, _ = attention_case([300], [100], 1, 1, 64, 32, torch.float16, 1, 3)
+    out, L, side = torch.zeros_like(q), kv4._load(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    a = kv4._Attn(q.data_ptr(), out.data_ptr(), *q.stride()[:2], *out.stride()[:2], start.data_ptr(), ln.data_ptr(), table.data_ptr(),
+                  1, q.shape[0], table.shape[1], 1, 1, 1, 0.125, 300, 100, None, 0)
+    for _ in range(50):
+        assert L.jepa_b200_kv4_attention_giving_up(c._ref, C.byref(a), 43, LIMIT, side.cuda_stream) == 0
+        told = 0
+        for k in range(20):
+            if k == 19:
+                side.synchronize()
+            try:
+                c.check()
+            except RuntimeError:
+                told += 1
+        assert told == 1
