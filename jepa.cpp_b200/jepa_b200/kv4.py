@@ -1,6 +1,7 @@
 """The paged 4-bit key / value cache on torch CUDA tensors: block tables and slot maps of a step, store, load, and the
 attention that reads the cache (include/jepa_b200.h, the kv4 block). Every call runs on the current stream of the
-tensors' device, without a synchronisation, and can be captured into a CUDA graph.
+tensors' device, without a synchronisation, and can be captured into a CUDA graph. There is no backward pass: rows that
+require grad are refused while autograd is on.
 
     cache = KV4Cache(n_pages, page_size, kv_heads, head_dim)
     t = build_tables(cached, added, table, free_pages, page_size, n_slots)   # new pages, slots, row ranges
@@ -170,6 +171,8 @@ class KV4Cache:
             raise ValueError(f"{name} must be [{n} rows, {heads}, {self.head_dim}]")
         if t.device != self._dev:
             raise ValueError(f"{name} must be on {self._dev}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} requires grad, and the 4-bit cache has no backward pass: detach it, or call under torch.no_grad()")
         stride = t.stride()
         if stride[2] != 1:
             raise ValueError(f"{name}'s channels must be contiguous")

@@ -143,3 +143,15 @@ def test_many_requests_over_wide_tables_with_unknown_bounds():
             check(out[r * n:(r + 1) * n, 0], o, bound(o, mean, size, torch.float16), f"request {r}")
     half = torch.finfo(torch.float16).eps / 2
     assert ((a - b).abs().double() <= 2 * half * b.abs().double() + 2 * 2.0 ** -11 * float(v.abs().max())).all()
+
+
+def test_rows_that_require_grad_are_refused():
+    c = kv4.KV4Cache(4, 16, 2, 64)
+    x = torch.randn(3, 2, 64, device="cuda").half().requires_grad_()
+    slots, start, ln, table = torch.arange(3, device="cuda"), i32([0, 3]), i32([3]), i32([[0]])
+    for call in (lambda a: c.store(a, a.detach(), slots), lambda a: c.store(a.detach(), a, slots), lambda a: c.attention(a, start, ln, table),
+                 lambda a: c.attention(a.detach(), start, ln, table, out=a * 1)):
+        with pytest.raises(ValueError, match="requires grad"):
+            call(x)
+        with torch.no_grad():
+            call(x)

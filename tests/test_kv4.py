@@ -125,3 +125,16 @@ def test_torch_view_refuses_what_is_not_on_a_gpu():
         kv4.KV4Cache.wrap(torch.zeros(4, 2, 2, 16, dtype=torch.uint8), torch.zeros(4, 2, 2, 2, 16, dtype=torch.float16))
     with pytest.raises(RuntimeError, match="head_dim 80"):
         kv4.KV4Cache(4, 16, 2, 80, device="cpu")
+
+
+def test_torch_view_refuses_rows_that_require_grad():
+    """Codes have no gradient: a row that autograd follows would lose it without a word."""
+    c = kv4.KV4Cache.__new__(kv4.KV4Cache)
+    c.head_dim, c.kv_heads, c._dev = 64, 2, torch.device("cpu")
+    x = torch.zeros(3, 2, 64, requires_grad=True)
+    for t in (x, x * 2, (x * 2).half()):
+        with pytest.raises(ValueError, match="k requires grad"):
+            c._rows(t, "k", 3, 2)
+        assert c._rows(t.detach(), "k", 3, 2) == (128, 64, 1)
+        with torch.no_grad():
+            assert c._rows(t, "k", 3, 2) == (128, 64, 1)
