@@ -56,6 +56,21 @@ bool pool_of(const char * fn, const jepa_b200_kv4_cache * c, jb::Kv4Pool & p) {
     return true;
 }
 
+// whether two of the rows x heads pieces of hd channels share an element; both strides are at least hd where they count
+bool pieces_overlap(long long rows, long long tok, long long heads, long long head, int hd) {
+    typedef __int128 wide;
+    if (rows < 2 || heads < 2 || tok >= (wide) (heads - 1) * head + hd || head >= (wide) (rows - 1) * tok + hd) return false;
+    // neither lies inside the other's steps: the closest rows to every head, from both sides
+    for (long long h = 1; h < heads; h++) {
+        const wide x = (wide) h * head, below = x / tok;
+        for (wide r = below; r <= below + 1; r++) {
+            const wide gap = r * tok - x;
+            if (r >= 1 && r < rows && gap < hd && gap > -hd) return true;
+        }
+    }
+    return false;
+}
+
 bool attn_of(const char * fn, const jb::Kv4Pool & p, const jepa_b200_kv4_attn * x, jb::Kv4Attn & a) {
     if (!x) { log("jepa: %s: the arguments are null\n", fn); return false; }
     if (x->type != jb::KV4_F16 && x->type != jb::KV4_BF16) { log("jepa: %s: type %u is not 1 (f16) or 30 (bf16)\n", fn, x->type); return false; }
@@ -74,6 +89,10 @@ bool attn_of(const char * fn, const jb::Kv4Pool & p, const jepa_b200_kv4_attn * 
     if (x->q_tok < 0 || x->q_head < 0 || x->o_tok < 0 || x->o_head < 0) { log("jepa: %s: strides must not be negative\n", fn); return false; }
     if (x->n_rows > 1 && x->o_tok < p.hd) { log("jepa: %s: rows of out overlap (stride %lld of %d channels)\n", fn, (long long) x->o_tok, p.hd); return false; }
     if (x->n_heads > 1 && x->o_head < p.hd) { log("jepa: %s: heads of out overlap (stride %lld of %d channels)\n", fn, (long long) x->o_head, p.hd); return false; }
+    if (pieces_overlap(x->n_rows, x->o_tok, x->n_heads, x->o_head, p.hd)) {
+        log("jepa: %s: rows and heads of out overlap (strides %lld and %lld)\n", fn, (long long) x->o_tok, (long long) x->o_head);
+        return false;
+    }
     a.q = x->q; a.out = x->out;
     a.q_tok = x->q_tok; a.q_head = x->q_head; a.o_tok = x->o_tok; a.o_head = x->o_head;
     a.q_start = x->q_start; a.lens = x->lens; a.table = x->table;

@@ -73,3 +73,30 @@ def test_refused_plans():
     assert L.jepa_b200_kv4_attention_plan(C.byref(c), C.byref(_attn()), None) == -1 and "result's pointer" in _err()
     assert L.jepa_b200_kv4_attention_plan(C.byref(c), C.byref(_attn(frame=-1)), out) == -1 and "frame" in _err()
     assert L.jepa_b200_kv4_attention_plan(None, C.byref(_attn()), out) == -1 and "cache is null" in _err()
+
+
+def test_out_overlaps():
+    """Refused exactly where two (row, head) pieces of out share an element."""
+    L, out = kv4._load(), (C.c_int * 4)()
+    c = _cache(kv_heads=1, head_dim=32)
+    rng = random.Random(5)
+    seen = {True: 0, False: 0}
+    for _ in range(3000):
+        rows, heads = rng.randint(1, 6), rng.randint(1, 6)
+        tok, head = rng.randint(30, 300), rng.randint(30, 300)
+        if rng.random() < 0.4:
+            tok, head = rng.randint(1, 8) * 32, rng.randint(1, 8) * 32
+        at = sorted(r * tok + h * head for r in range(rows) for h in range(heads))
+        overlap = any(b - a < 32 for a, b in zip(at, at[1:]))
+        rc = L.jepa_b200_kv4_attention_plan(C.byref(c), C.byref(_attn(n_rows=rows, n_heads=heads, o_tok=tok, o_head=head)), out)
+        assert rc == (-1 if overlap else 0), (rows, heads, tok, head)
+        assert not overlap or "overlap" in _err()
+        seen[overlap] += 1
+    assert min(seen.values()) > 500
+    # the far ends: strides and counts whose products pass 63 bits
+    big = 1 << 62
+    for kw, rc in ((dict(n_rows=1 << 14, n_heads=65535, o_tok=big, o_head=big), -1), (dict(n_rows=1 << 14, n_heads=65535, o_tok=big, o_head=32), 0),
+                   (dict(n_rows=1 << 14, n_heads=65535, o_tok=65535 * 32, o_head=32), 0), (dict(n_rows=1 << 14, n_heads=65535, o_tok=65535 * 32 - 1, o_head=32), -1),
+                   (dict(n_rows=1 << 14, n_heads=65535, o_tok=32, o_head=32 << 14), 0), (dict(n_rows=1 << 14, n_heads=65535, o_tok=33, o_head=32 << 14), -1)):
+        assert L.jepa_b200_kv4_attention_plan(C.byref(c), C.byref(_attn(**kw)), out) == rc, kw
+        L.jepa_error_reset()
