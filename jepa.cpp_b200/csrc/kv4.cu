@@ -258,7 +258,6 @@ double row_bytes(const Kv4Pool & p, int type) {
 int kv4_store(const Kv4Pool & p, const Kv4Rows & r, int type, const int64_t * slots, long long n, cudaStream_t st) {
     if (n < 1) return 0;
     const long long blocks = ((n + 7) / 8 * p.heads + 3) / 4;
-    if (blocks > 0x7fffffffLL) { log("jepa: jepa_b200_kv4_store: %lld tokens are too many for one call\n", n); return -1; }
     KTimer kt("kv4_store", st, 0, row_bytes(p, type) * n);
     const dim3 grid((unsigned) blocks);
     switch (type) {
@@ -272,7 +271,6 @@ int kv4_load(const Kv4Pool & p, const Kv4Rows & r, int type, const int64_t * slo
     if (n < 1) return 0;
     const int tok = type == KV4_F32 ? load_tokens<float>() : load_tokens<__half>();
     const long long blocks = ((n + tok - 1) / tok * p.heads + 3) / 4;
-    if (blocks > 0x7fffffffLL) { log("jepa: jepa_b200_kv4_load: %lld tokens are too many for one call\n", n); return -1; }
     KTimer kt("kv4_load", st, 0, row_bytes(p, type) * n);
     const dim3 grid((unsigned) blocks);
     switch (type) {

@@ -128,6 +128,14 @@ int attention(const char * fn, const jepa_b200_kv4_cache * cache, const jepa_b20
     return jb::kv4_attention(p, a, (cudaStream_t) stream);
 }
 
+// tokens of a store or load: a block takes 16 (token, head) pairs at least, and a grid has 2^31 - 1 blocks
+bool token_count(const char * fn, const jb::Kv4Pool & p, int64_t n) {
+    const int64_t most = (0x7fffffffLL / p.heads - 1) * 16;
+    if (n >= 0 && n <= most) return true;
+    log("jepa: %s: %lld tokens are out of range (0 .. %lld for %d heads)\n", fn, (long long) n, (long long) most, p.heads);
+    return false;
+}
+
 }  // namespace
 
 extern "C" {
@@ -167,10 +175,8 @@ int jepa_b200_kv4_store(const jepa_b200_kv4_cache * cache, const void * k, const
     static const char * fn = "jepa_b200_kv4_store";
     jb::Kv4Pool p;
     if (!pool_of(fn, cache, p) || !row_type(fn, type)) return -1;
-    if (n_tokens < 0 || k_tok < 0 || k_head < 0 || v_tok < 0 || v_head < 0) {
-        log("jepa: %s: %lld tokens and the strides must not be negative\n", fn, (long long) n_tokens);
-        return -1;
-    }
+    if (!token_count(fn, p, n_tokens)) return -1;
+    if (k_tok < 0 || k_head < 0 || v_tok < 0 || v_head < 0) { log("jepa: %s: strides must not be negative\n", fn); return -1; }
     if (!n_tokens) return 0;
     const unsigned size = type == jb::KV4_F32 ? 4 : 2;
     if (device_pointers(fn, {{"cache.q", p.q, 16}, {"cache.d", p.d, 16}, {"k", k, size}, {"v", v, size}, {"slots", slots, 8}})) return -1;
@@ -182,7 +188,7 @@ int jepa_b200_kv4_load(const jepa_b200_kv4_cache * cache, const int64_t * slots,
     static const char * fn = "jepa_b200_kv4_load";
     jb::Kv4Pool p;
     if (!pool_of(fn, cache, p) || !row_type(fn, type)) return -1;
-    if (n_tokens < 0) { log("jepa: %s: %lld tokens\n", fn, (long long) n_tokens); return -1; }
+    if (!token_count(fn, p, n_tokens)) return -1;
     if (!n_tokens) return 0;
     if (device_pointers(fn, {{"cache.q", p.q, 16}, {"cache.d", p.d, 16}, {"k", k, 16}, {"v", v, 16}, {"slots", slots, 8}})) return -1;
     return jb::kv4_load(p, {k, v, 0, 0, 0, 0}, (int) type, slots, n_tokens, (cudaStream_t) stream);

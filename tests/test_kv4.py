@@ -138,3 +138,16 @@ def test_torch_view_refuses_rows_that_require_grad():
         assert c._rows(t.detach(), "k", 3, 2) == (128, 64, 1)
         with torch.no_grad():
             assert c._rows(t, "k", 3, 2) == (128, 64, 1)
+
+
+@pytest.mark.parametrize("heads", [1, 3, 8, 1024])
+def test_more_tokens_than_a_grid_holds_are_refused(heads):
+    L = kv4._load()
+    r = C.byref(_cache(kv_heads=heads))
+    most = (0x7fffffff // heads - 1) * 16
+    assert -(-(-(-most // 4) * heads) // 4) <= 0x7fffffff         # blocks of four warps, four tokens of one head each
+    for n in (most + 1, 1 << 40, 1 << 60, (1 << 61) + 8, (1 << 63) - 7, (1 << 63) - 1):
+        assert L.jepa_b200_kv4_store(r, PTR, PTR, 1, 128, 64, 128, 64, PTR, n, None) == -1 and "out of range" in _err()
+        assert L.jepa_b200_kv4_load(r, PTR, n, PTR, PTR, 0, None) == -1 and "out of range" in _err()
+    # the largest count comes as far as the pointers
+    assert L.jepa_b200_kv4_store(r, None, PTR, 1, 128, 64, 128, 64, PTR, most, None) == -1 and "k is null" in _err()
