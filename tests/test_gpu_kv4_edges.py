@@ -13,9 +13,10 @@ pytestmark = pytest.mark.gpu
 NAN = float("nan")
 
 
-def masked_case(lens, new, heads, kv_heads, dim, page, dtype, frame, seed, gone=(), broken=()):
+def masked_case(lens, new, heads, kv_heads, dim, page, dtype, frame, seed, gone=(), broken=(), broken_keys=()):
     """Like attention_case, with the pages of the (request, page index) pairs `gone` taken out of the table, and the value
-    scale of group 0 of the (request, key) pairs `broken` not a number. ref holds NaN where a row sees such a key."""
+    scale of group 0 of the (request, key) pairs `broken`, the key scale of the last group of `broken_keys`, not a number. ref
+    holds NaN where a row sees such a key: in the first 32 channels, or in all of them."""
     c, q, start, ln, table, _, _ = attention_case(lens, new, heads, kv_heads, dim, page, dtype, frame, seed)
     t = table.cpu().tolist()
     T = sum(new)
@@ -25,7 +26,7 @@ def masked_case(lens, new, heads, kv_heads, dim, page, dtype, frame, seed, gone=
         slots = torch.tensor([t[r][j // page] * page + j % page for j in range(L)], dtype=torch.int64)
         k, v = (x.double().cpu() for x in c.load(slots.cuda(), torch.float32))
         held = torch.tensor([(r, j // page) not in gone for j in range(L)], dtype=torch.bool)
-        bad = torch.tensor([(r, j) in broken for j in range(L)], dtype=torch.bool)
+        bad, bad_key = (torch.tensor([(r, j) in where for j in range(L)], dtype=torch.bool) for where in (broken, broken_keys))
         pos = torch.arange(L - n, L)
         lim = torch.full_like(pos, L)
         if frame:
@@ -43,12 +44,15 @@ def masked_case(lens, new, heads, kv_heads, dim, page, dtype, frame, seed, gone=
             o = p @ vv
             tol[at:at + n, h] = bound(o, mean, size, dtype)
             o[(see & bad).any(1), :32] = NAN
+            o[(see & bad_key).any(1)] = NAN
             ref[at:at + n, h] = o
         at += n
     for r, i in gone:
         table[r, i] = -3 if (r + i) % 2 else c.n_pages + i
     for r, j in broken:
         c.d[t[r][j // page], 1, :, 0, j % page] = NAN
+    for r, j in broken_keys:
+        c.d[t[r][j // page], 0, :, -1, j % page] = NAN
     return c, q, start, ln, table, ref, tol
 
 
@@ -155,3 +159,59 @@ def test_rows_that_require_grad_are_refused():
             call(x)
         with torch.no_grad():
             call(x)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, torch.float16), (128, torch.bfloat16), (32, torch.float16), (96, torch.bfloat16)])
+@pytest.mark.parametrize("lens,new,heads,kv_heads", [
+    ([70], [9], 1, 1), ([70, 90], [1, 16], 1, 1),                # one tile of 8 columns, two
+    ([300], [30], 2, 2), ([300, 90], [4, 1], 14, 2),             # two passes over the columns; grouped heads
+    ([400], [258], 1, 1), ([500, 80], [259, 3], 2, 2),           # whole tiles of 256 and 2 or 3 columns left over
+    ([2600], [6], 2, 1), ([2600], [70], 2, 1),                   # several ranges of keys, joined at the end: few rows, many
+    ([330], [40], 3, 1)])
+def test_scales_that_are_not_numbers_reach_the_rows_that_see_them_and_no_other(lens, new, heads, kv_heads, dim, dtype):
+    """A value scale, a key scale and a page that is not there, each among the keys that the rows of a causal chunk begin
+    to see one after the other: NaN in the channels that they give, from the first row that sees them on, in both kernels."""
+    page = 16
+    broken = {(r, L - n + n // 2) for r, (L, n) in enumerate(zip(lens, new))}
+    keys = {(r, L - 1 - n // 4) for r, (L, n) in enumerate(zip(lens, new)) if n > 4}
+    gone = {(r, 1) for r in range(len(lens))}
+    for frame in (1, 0):
+        c, q, start, ln, table, ref, tol = masked_case(lens, new, heads, kv_heads, dim, page, dtype, frame, sum(lens) + dim, gone, broken, keys)
+        assert ref.isnan().any() and (frame == 0 or max(new) < 5 or not ref.isnan().all(-1).all())
+        for bounds in (dict(max_len=max(lens), max_new=max(new)), {}, dict(max_len=1, max_new=1)):
+            check_nan(c.attention(q, start, ln, table, frame=frame, **bounds), ref, tol, str(bounds))
+    # behind every row's mask: in the last page, past the last key
+    c, q, start, ln, table, ref, tol = masked_case(lens, new, heads, kv_heads, dim, page, dtype, 1, sum(lens) + dim)
+    assert not ref.isnan().any()
+    check_nan(c.attention(q, start, ln, table, frame=1, max_new=max(new)), ref, tol)
+
+
+@pytest.mark.parametrize("dtype,big", [(torch.bfloat16, 2.0 ** 40), (torch.bfloat16, 2.0 ** 90), (torch.bfloat16, 2.0 ** 118), (torch.float16, 2.0 ** 12),
+                                       (torch.bfloat16, 2.0 ** 14)])
+@pytest.mark.parametrize("n,lens", [(1, [700, 90]), (9, [2500, 64]), (40, [700, 90]), (300, [1500, 400])])
+def test_a_huge_query_takes_the_value_of_its_key(n, lens, dtype, big):
+    """Row i is the cached key t_i times 2^12 .. 2^118: the score of t_i is above every other by 2^8 and more, its weight is all
+    there is, and the row is its value: off by the value's rounding to the type and, where weights go into the product
+    rounded to f16 and into the sum as they are, by 2^-11 of it."""
+    heads, kv_heads, dim, page = 2, 1, 64, 32
+    c, _, start, ln, table, _, _ = attention_case(lens, [n, n], heads, kv_heads, dim, page, dtype, 1, 77)
+    t = table.cpu().tolist()
+    q, want = torch.zeros(2 * n, heads, dim, dtype=torch.float64), torch.zeros(2 * n, heads, dim, dtype=torch.float64)
+    for r, L in enumerate(lens):
+        slots = torch.tensor([t[r][j // page] * page + j % page for j in range(L)], device="cuda")
+        k, v = (x[:, 0].double().cpu() for x in c.load(slots, torch.float32))
+        dots = k @ k.T
+        margin = dots.diag() - (dots - torch.diag(dots.diag() * 2)).amax(1)
+        for i in range(n):
+            seen = L - n + i + 1                                  # causal: keys that the row sees
+            for h in range(heads):
+                j = int(margin[:seen].sub(1e-3 * ((torch.arange(seen) * 37 + 11 * i + h) % 97)).argmax()) if i % 3 else seen - 1
+                if margin[j] <= 4:
+                    j = int(margin[:seen].argmax())
+                assert margin[j] > 4                              # x 2^12 / sqrt(64): 2^11 apart
+                q[r * n + i, h], want[r * n + i, h] = (k[j] * big).to(dtype).double(), v[j]
+    assert torch.isfinite(q).all()
+    half = torch.finfo(dtype).eps / 2
+    for bounds in (dict(max_len=max(lens), max_new=n), {}):
+        out = c.attention(q.to(dtype).cuda(), start, ln, table, frame=1, **bounds).double().cpu()
+        assert ((out - want).abs() <= (half + 2.0 ** -11) * want.abs() + 1e-30).all()
