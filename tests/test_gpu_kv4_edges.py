@@ -215,3 +215,47 @@ def test_a_huge_query_takes_the_value_of_its_key(n, lens, dtype, big):
     for bounds in (dict(max_len=max(lens), max_new=n), {}):
         out = c.attention(q.to(dtype).cuda(), start, ln, table, frame=1, **bounds).double().cpu()
         assert ((out - want).abs() <= (half + 2.0 ** -11) * want.abs() + 1e-30).all()
+
+
+_FIRST_CALLS = r"""
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+from jepa_b200 import kv4
+dev, page, dim, n = "cuda", 32, 64, [1, 3, 300]
+i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+c = kv4.KV4Cache(120, page, 2, dim)
+cached, added, table, free = i32([0, 40, 1500]), i32(n), torch.arange(3 * 64, dtype=torch.int32, device=dev).view(3, 64) % 56, i32(list(range(56, 120)))
+start_table = table.clone()
+g = torch.Generator(dev).manual_seed(1)
+k, v = (torch.randn(sum(n), 2, dim, generator=g, device=dev).half() for _ in range(2))
+q = torch.randn(sum(n), 4, dim, generator=g, device=dev).half()
+
+def step():
+    t = kv4.build_tables(cached, added, table, free, page, sum(n))
+    c.store(k, v, t.slots)
+    return (c.attention(q, t.q_start, t.lens, table, frame=1, max_len=1800, max_new=300), *c.load(t.slots), t.slots, t.state)
+
+side = torch.cuda.Stream()
+side.wait_stream(torch.cuda.current_stream())
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=side):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+got = [x.clone() for x in got]
+table.copy_(start_table)
+want = step()
+c.check()
+assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[4].tolist()[0] == 0 and bool((got[0] != 0).any())
+print("SAME")
+"""
+
+
+def test_the_first_calls_of_a_process_can_be_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "jepa.cpp_b200")
+    r = subprocess.run([sys.executable, "-c", _FIRST_CALLS, root], capture_output=True, text=True, timeout=180)
+    assert r.returncode == 0 and "SAME" in r.stdout, r.stderr[-2000:]
