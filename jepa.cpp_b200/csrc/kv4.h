@@ -70,12 +70,15 @@ struct Kv4Attn {
     int type;
     void * ws;
     size_t ws_bytes;
-    long long wait_limit = 4000000000LL;    // cycles before a wait of the tiles kernel gives up (about 2 s)
-    int give_up_at = 0;                     // the wait (by its code) that gives up at once: the failure path's test
+};
+// the bounded waits of the tiles kernel
+struct Kv4Waits {
+    long long limit = 4000000000LL;         // cycles before one gives up (about 2 s)
+    int give_up_at = 0;                     // the one (by its code) that gives up at once: the failure path's test
 };
 size_t kv4_attention_workspace(const Kv4Pool & p, const Kv4Attn & a);
 void kv4_attention_plan(const Kv4Pool & p, const Kv4Attn & a, int * out);      // see jepa_b200_kv4_attention_plan
-int kv4_attention(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st);
+int kv4_attention(const Kv4Pool & p, const Kv4Attn & a, const Kv4Waits & w, cudaStream_t st);
 // Waits for the stream: the wait that ran out in a kernel of the current device, if one did that no call has told yet; 0, or -1: not read
 int kv4_error_flag(cudaStream_t st);
 

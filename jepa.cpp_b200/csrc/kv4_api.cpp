@@ -112,9 +112,9 @@ bool row_type(const char * fn, uint32_t type) {
     return false;
 }
 
-// `a` comes with the limits of its waits
-int attention(const char * fn, const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, jb::Kv4Attn a, void * stream) {
+int attention(const char * fn, const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, const jb::Kv4Waits & waits, void * stream) {
     jb::Kv4Pool p;
+    jb::Kv4Attn a;
     if (!pool_of(fn, cache, p) || !attn_of(fn, p, args, a)) return -1;
     if (!a.n_req || !a.n_rows) return 0;
     const size_t need = jb::kv4_attention_workspace(p, a);
@@ -125,7 +125,7 @@ int attention(const char * fn, const jepa_b200_kv4_cache * cache, const jepa_b20
     const void * ws = need ? a.ws : p.q;
     if (device_pointers(fn, {{"cache.q", p.q, 16}, {"cache.d", p.d, 16}, {"q", a.q, 2}, {"out", a.out, 2}, {"q_start", a.q_start, 4},
                              {"lens", a.lens, 4}, {"table", a.table, 4}, {"workspace", ws, 16}})) return -1;
-    return jb::kv4_attention(p, a, (cudaStream_t) stream);
+    return jb::kv4_attention(p, a, waits, (cudaStream_t) stream);
 }
 
 // tokens of a store or load: a block takes 16 (token, head) pairs at least, and a grid has 2^31 - 1 blocks
@@ -213,7 +213,7 @@ int jepa_b200_kv4_attention_plan(const jepa_b200_kv4_cache * cache, const jepa_b
 }
 
 int jepa_b200_kv4_attention(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, void * stream) {
-    return attention("jepa_b200_kv4_attention", cache, args, jb::Kv4Attn(), stream);
+    return attention("jepa_b200_kv4_attention", cache, args, jb::Kv4Waits(), stream);
 }
 
 int jepa_b200_kv4_attention_giving_up(const jepa_b200_kv4_cache * cache, const jepa_b200_kv4_attn * args, int wait, long long limit_cycles,
@@ -223,10 +223,10 @@ int jepa_b200_kv4_attention_giving_up(const jepa_b200_kv4_cache * cache, const j
         log("jepa: %s: need 40 <= wait <= 51 and 1 <= limit_cycles <= 4e9 (%d, %lld)\n", fn, wait, limit_cycles);
         return -1;
     }
-    jb::Kv4Attn a;
-    a.wait_limit = limit_cycles;
-    a.give_up_at = wait;
-    return attention(fn, cache, args, a, stream);
+    jb::Kv4Waits waits;
+    waits.limit = limit_cycles;
+    waits.give_up_at = wait;
+    return attention(fn, cache, args, waits, stream);
 }
 
 int jepa_b200_kv4_check(void * stream) {

@@ -545,7 +545,7 @@ int rows_launch(const Kv4Pool & p, const Kv4Attn & a, const Plan & r, int vec, c
 }
 
 template <class T, int NG>
-int launch(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st) {
+int launch(const Kv4Pool & p, const Kv4Attn & a, const Kv4Waits & waits, cudaStream_t st) {
     Plan r = plan_of(p, a);
     if (r.sp.n_split > 1) {
         r.sp.o = (float *) a.ws;
@@ -555,7 +555,7 @@ int launch(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st) {
     const int vec = (((uintptr_t) a.q & 15) == 0 && ((a.q_tok | a.q_head) & 7) == 0 ? 1 : 0) |
                     (((uintptr_t) a.out & 7) == 0 && ((a.o_tok | a.o_head) & 3) == 0 ? 2 : 0) |
                     (((uintptr_t) a.out & 15) == 0 && ((a.o_tok | a.o_head) & 7) == 0 ? 4 : 0);
-    if (r.tc && kv4_tiles(p, a, r.sp, r.tiles, vec, st)) return -1;
+    if (r.tc && kv4_tiles(p, a, waits, r.sp, r.tiles, vec, st)) return -1;
     if (r.nt == 1 ? rows_launch<T, NG, 1>(p, a, r, vec, st) : rows_launch<T, NG, 2>(p, a, r, vec, st)) return -1;
     if (r.sp.n_split > 1) {
         // (a CTA walks rows of its request from its own on: max_new may be unknown, and then far too many)
@@ -566,12 +566,12 @@ int launch(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st) {
 }
 
 template <class T>
-int launch_dim(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st) {
+int launch_dim(const Kv4Pool & p, const Kv4Attn & a, const Kv4Waits & waits, cudaStream_t st) {
     switch (p.hd / 32) {
-        case 1: return launch<T, 1>(p, a, st);
-        case 2: return launch<T, 2>(p, a, st);
-        case 3: return launch<T, 3>(p, a, st);
-        default: return launch<T, 4>(p, a, st);
+        case 1: return launch<T, 1>(p, a, waits, st);
+        case 2: return launch<T, 2>(p, a, waits, st);
+        case 3: return launch<T, 3>(p, a, waits, st);
+        default: return launch<T, 4>(p, a, waits, st);
     }
 }
 
@@ -590,9 +590,9 @@ void kv4_attention_plan(const Kv4Pool & p, const Kv4Attn & a, int * out) {
     out[3] = r.sp.chunk;
 }
 
-int kv4_attention(const Kv4Pool & p, const Kv4Attn & a, cudaStream_t st) {
+int kv4_attention(const Kv4Pool & p, const Kv4Attn & a, const Kv4Waits & w, cudaStream_t st) {
     KTimer kt("kv4_attention", st);
-    return a.type == KV4_F16 ? launch_dim<__half>(p, a, st) : launch_dim<__nv_bfloat16>(p, a, st);
+    return a.type == KV4_F16 ? launch_dim<__half>(p, a, w, st) : launch_dim<__nv_bfloat16>(p, a, w, st);
 }
 
 }  // namespace jb

@@ -145,13 +145,15 @@ __device__ __forceinline__ bool elect_one() {
     return r != 0;
 }
 
+struct Args : Kv4Attn { Kv4Waits waits; };
+
 // the whole warp waits, and agrees on the outcome
-__device__ __forceinline__ bool warp_wait(const Kv4Attn & a, uint64_t * bar, uint32_t parity, int code) {
-    if (code == a.give_up_at) {
+__device__ __forceinline__ bool warp_wait(const Args & a, uint64_t * bar, uint32_t parity, int code) {
+    if (code == a.waits.give_up_at) {
         atomicExch(&g_kv4_failures.code, code);
         return false;
     }
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, code, &g_kv4_failures.code, a.wait_limit));
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, code, &g_kv4_failures.code, a.waits.limit));
 }
 
 // bits of an f16 infinity or NaN
@@ -163,7 +165,7 @@ template <int NG> __host__ __device__ constexpr int atoms() { return (NG + 1) / 
 template <int NG> constexpr size_t tiles_smem() { return (size_t) atoms<NG>() * ((NG <= 2 ? 0 : 2 * QATOM) + 2 * STAGES * ATOM) + 1024; }
 
 template <class T, int NG>
-__global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, const Kv4Attn a, const Split sp, int tiles, int vec) {
+__global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, const Args a, const Split sp, int tiles, int vec) {
     constexpr int HD = 32 * NG, AT = atoms<NG>(), W = 4 * NG;      // W: 8-channel words of a row
     constexpr bool QT = NG <= 2;                                   // Q in tensor memory, else in shared memory
     constexpr int NB = 2;                                          // buffers of S a tile
@@ -662,7 +664,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
 }
 
 template <class T, int NG>
-int launch(const Kv4Pool & p, const Kv4Attn & a, const Split & sp, int tiles, int vec, cudaStream_t st) {
+int launch(const Kv4Pool & p, const Args & a, const Split & sp, int tiles, int vec, cudaStream_t st) {
     if (allow_smem<k_kv4_tiles<T, NG>>((int) tiles_smem<NG>())) return -1;
     const dim3 grid((unsigned) sp.n_split, (unsigned) (p.heads * tiles), (unsigned) a.n_req);
     JB_CUDA(launch_pdl(k_kv4_tiles<T, NG>, grid, dim3(THREADS), tiles_smem<NG>(), st, p, a, sp, tiles, vec));
@@ -670,7 +672,7 @@ int launch(const Kv4Pool & p, const Kv4Attn & a, const Split & sp, int tiles, in
 }
 
 template <class T>
-int launch_dim(const Kv4Pool & p, const Kv4Attn & a, const Split & sp, int tiles, int vec, cudaStream_t st) {
+int launch_dim(const Kv4Pool & p, const Args & a, const Split & sp, int tiles, int vec, cudaStream_t st) {
     switch (p.hd / 32) {
         case 1: return launch<T, 1>(p, a, sp, tiles, vec, st);
         case 2: return launch<T, 2>(p, a, sp, tiles, vec, st);
@@ -698,7 +700,8 @@ int kv4_error_flag(cudaStream_t st) {
     return 0;
 }
 
-int kv4_tiles(const Kv4Pool & p, const Kv4Attn & a, const Split & sp, int tiles, int vec, cudaStream_t st) {
+int kv4_tiles(const Kv4Pool & p, const Kv4Attn & attn, const Kv4Waits & waits, const Split & sp, int tiles, int vec, cudaStream_t st) {
+    const Args a{attn, waits};
     return a.type == KV4_F16 ? launch_dim<__half>(p, a, sp, tiles, vec, st) : launch_dim<__nv_bfloat16>(p, a, sp, tiles, vec, st);
 }
 

@@ -105,6 +105,6 @@ int allow_smem(int bytes) {
 }
 
 // The tiles kernel (kv4_attention_tc.cu): `grid` = (key ranges, cache heads x tiles of 256 columns, requests).
-int kv4_tiles(const Kv4Pool & p, const Kv4Attn & a, const Split & sp, int tiles, int vec, cudaStream_t st);
+int kv4_tiles(const Kv4Pool & p, const Kv4Attn & a, const Kv4Waits & waits, const Split & sp, int tiles, int vec, cudaStream_t st);
 
 }  // namespace jb
