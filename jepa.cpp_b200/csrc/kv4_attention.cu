@@ -240,8 +240,8 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
             read = read == (STAGES - 1) * SB ? 0 : read + SB;
             const __half * kd = (const __half *) (vb + STEP * RB), * vd = kd + NG * STEP;
             const int key = k0 + STEP * (WARPS * i + warp);
-            // two tiles of 16 keys, one after the other (side by side in one body of twice the length, the schedulers waited for
-            // instructions: 121 us for 64 sessions of 1000 .. 8190 keys)
+            // two tiles of 16 keys, one after the other (side by side in one body of twice the length: 142 us for 64 sessions of
+            // 1000 .. 8190 keys instead of 120, and the counters showed stalls for instructions)
 #pragma unroll 1
             for (int u = 0; u < 2; u++) {
                 // ---- scores
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 4 : 3) k_kv4_rows(const 
                             if (k >= min(lim[nt][e & 1], k1) || ((hole >> u) & 1)) s[nt][e] = -INFINITY;
                         }
                     }
-                    asm volatile("" ::: "memory");               // a branch, not selects in every step
+                    asm volatile("" ::: "memory");               // keeps the masks out of the steps that need none
                 }
                 float mx[NT][2];
                 bool raise = false;
@@ -520,8 +520,13 @@ Plan plan_of(const Kv4Pool & p, const Kv4Attn & a) {
     const long long total = ctas * p.heads * a.max_len, slots = r.tc ? 148 : 148 * 4;
     const long long whole = (a.max_len + 127LL) & ~127LL;
     long long chunk = (std::max(std::max(256LL, std::min(1024LL, total / slots)), total / (4 * slots)) + 127) & ~127LL;
-    // one range where a second would be short or small: it would cost a second kernel (516 keys of one session: 8 us, against
-    // 8 us in three ranges and 5 us of merge)
+    // One range where a second would be short or small: it would cost a second kernel, and for many rows their partial sums.
+    // One range against ranges of 256 keys, us, replayed one after the other: one row of 16 heads of 64, 300 / 516 / 768 keys,
+    // 1 session 5.5 / 7.1 / 7.6 and 7.0 / 7.2 / 7.2, 32 sessions 8.1 / 11.9 / 14.2 and 8.1 / 25.4 / 14.2; 8 cache heads of
+    // 128, 1 session 7.4 / 9.9 / 10.5 and 8.6 / 8.6 / 8.6, 32 sessions 9.2 / 13.8 / 15.5 and 24.0 / 31.7 / 28.7; 128 rows of 16
+    // heads of 64, 1 session 11.8 / 15.2 / 17.9 and 32.8 / 32.9 / 33.0. So at most 2 us are lost, where a single session has
+    // few cache heads and 500 keys and more. (Behind 768 keys many rows of few sessions pay for it: those 128 rows take
+    // 33 us at 800 keys, of 4 sessions 100 us instead of 18 at 768.)
     if (a.max_len <= 768 || a.max_len <= chunk + chunk / 4) chunk = whole;
     r.sp.chunk = (int) chunk;                                // at most `whole`, which is below 2^31 (attn_of)
     r.sp.n_split = (int) ((a.max_len + chunk - 1) / chunk);

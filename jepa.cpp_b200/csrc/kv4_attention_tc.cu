@@ -17,9 +17,11 @@
 // Up to head_dim 64 TMEM holds Q beside S and O, above that Q stays in shared memory. The tensor core reads shared memory, and A
 // in TMEM, at about 64 bytes a cycle each: a 128 x 64 x 16 product takes 64 cycles with Q in TMEM and 100 with Q in shared
 // memory, 128 x 128 x 16 (P V at head_dim 128) 64. What bounds it: at head_dim 128 the products, 2100 of the 2700 cycles a pair
-// of tiles takes for 64 keys (chunks of 700 .. 2047 rows behind 4100 .. 8191 keys, 32 / 8 heads: 730 us, 673 TFLOP/s); at
-// head_dim 64 the softmax, 1024 of 2300 cycles of which are exponentials (96 x 258 rows over 774 keys, 16 heads: 250 us
-// of 285, the rest is the rows kernel's for the last 2 rows).
+// of tiles takes for 64 keys (chunks of 700 .. 2047 rows behind 4100 .. 8191 keys, 32 / 8 heads: 698 us, 704 TFLOP/s); at
+// head_dim 64 the softmax, 1024 of 2300 cycles of which are exponentials, and what a CTA takes whatever its keys (queries,
+// tensor memory, first codes, stores): 96 x 256 rows of 16 heads take 91 us and 12 us for every 64 keys, 247 us for 774, which
+// is 17,000 cycles a CTA and 2250 for every 64 keys (258 rows: 287 us, the rows kernel takes the last 2).
+// Registers: 118 to 128, with 48 bytes of spills at head_dim 128 and 8 at 96.
 // Measured and not taken, at head_dim 128: 128 keys a block with one buffer of S, 784 us or more (the softmax waits 2200 cycles
 // a block); Q in TMEM with one buffer, 858; two blocks' scores in one product of N 128, 884; turns of the two tiles' exponentials,
 // 756 against 742; a quarter of the exponentials as polynomials, no change (head_dim 64: 301 instead of 312).
@@ -137,8 +139,7 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return r;
 }
 
-// one lane of a converged warp; the compiler keeps what the products need in uniform registers under it (under lane == 0 it
-// would not: a product then took 120 cycles to issue)
+// one lane of a converged warp (products issued under lane == 0 instead took 120 cycles each to issue)
 __device__ __forceinline__ bool elect_one() {
     uint32_t r;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
     __shared__ int abort_sh;
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    const int warp = __shfl_sync(0xffffffffu, (int) (threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // warp: uniform to the compiler
+    const int warp = __shfl_sync(0xffffffffu, (int) (threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int kh = blockIdx.y / tiles, r = blockIdx.z, G = a.heads / pool.heads;
     const Req rq = request_of(a, pool.page_shift, r);
     const int n_cols = tile_columns((rq.row1 - rq.row0) * G);
@@ -311,20 +312,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_tiles(const Kv4Pool pool, co
             const uint32_t d_plane = ((uint32_t) pool.heads * NG) << pool.page_shift, q_page = ((uint32_t) pool.heads << pool.page_shift) * 32 * NG;
             const uint8_t * q_head = pool.q + kv4_q_at(pool, 0, keys ? 0 : 1, kh, 0);
             const uint16_t * d_head = (const uint16_t *) pool.d + kv4_d_at(pool, 0, keys ? 0 : 1, kh, 0);
-            // (a table entry is loaded a block before it is used and checked: volatile, or the compiler puts the load off to
-            // its use, and the block waits for it)
+            // (a table entry is loaded a block before it is used and checked; volatile keeps the load there. With this, the scales
+            // in 32 bits each and no choice of values behind the loads, chunks took 711 us instead of 742, frames 311 instead of 334)
             auto entry_at = [&](int key) -> int { return key < kend ? *(const volatile int32_t *) (table + (key >> pool.page_shift)) : -1; };
             uint4 raw[NG], next[NG];                            // this block's row and the next one's
-            // their scales (vd, K warps: those of the value, for the masks); in 32 bits each: pairs of 16 would be put
-            // together, and waited for, as soon as they are loaded
+            // their scales (vd, K warps: those of the value, for the masks)
             uint32_t d[NG], dn[NG], vd[NG], vdn[NG];
             int entry = entry_at(k0 + kt), heldn = -1;          // table entry of the block to be loaded; page of the one in `next`
             auto load = [&](int j) {
                 const int key = k0 + j * BLK + kt;
                 const int page = (uint32_t) entry < (uint32_t) n_pages ? entry : -1;
                 heldn = page;
-                // (a row without a page loads page 0's, and its scales become 0 at its use: a branch, or a choice of values
-                // here, would wait for the loads)
+                // (a row without a page loads page 0's, and its scales become 0 at its use)
                 const uint4 * q = (const uint4 *) (q_head + (uint64_t) (uint32_t) max(page, 0) * q_page + (key & pmask) * 16 * NG);
                 const uint16_t * s = d_head + (uint64_t) (uint32_t) max(page, 0) * (2 * d_plane) + (key & pmask);
 #pragma unroll

@@ -63,8 +63,11 @@ __device__ __forceinline__ int visible(const Req & q, int row, int frame) {
 // Columns of a request and cache head that the tiles kernel takes, of n in all: whole tiles of 256, and what is left over if
 // it is more than 32; the rows kernel takes the rest, 16 at a time. 32 sessions of 6000 .. 8000 keys, 4 cache heads, head_dim 64 / 128:
 // 24 columns take the rows kernel 90 / 137 us and the tiles kernel 135 / 197, 32 columns 101 / 150 and 141 / 204; a third
-// and fourth pass over the cache would cost more than the tiles kernel, whose time hardly depends on the columns. (258
-// columns in two CTAs of the tiles kernel: the second, for 2 of them, took as long as the first.)
+// and fourth pass over the cache would cost more than the tiles kernel there: 40 / 48 / 64 columns of 32 sessions of 7000 keys,
+// 16 heads of 64, 579 / 631 / 403 us against 387. (258 columns in two CTAs of the tiles kernel: the second, for 2 of
+// them, took as long as the first.) The border costs something on either side: 32 columns of those 32 sessions of 16 heads
+// take 442 us and would take 387 as tiles; 40 and 48 columns of 1 to 8 sessions would mostly be 5 to 40 % faster in the rows
+// kernel (one session of 500 keys, 16 heads of 64: 7.8 us against 13.6; 4000 keys, 8 heads of 128: 17.9 against 21.0).
 constexpr int FEW = 32;
 __host__ __device__ inline int tile_columns(int n) { return n % 256 > FEW ? n : n - n % 256; }
 

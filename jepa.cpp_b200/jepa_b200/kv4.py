@@ -208,8 +208,8 @@ class KV4Cache:
         """Attention of the rows q [rows, heads, head_dim] (f16 or bf16) over the cached rows of their requests:
         request r owns rows q_start[r] .. q_start[r + 1] - 1 and the first lens[r] positions of table[r]. frame: 0 =
         every cached key, 1 = causal, F = block-causal over frames of F tokens. max_len / max_new: bounds of lens and of
-        a request's rows, which the launch is laid out for (they change no result). out (zeros by default) keeps the
-        rows of no request."""
+        a request's rows, which the launch is laid out for (they change no result beyond its rounding). out (zeros by
+        default) keeps the rows of no request; it must not overlap q."""
         _need(isinstance(q, torch.Tensor) and q.dim() == 3, "q must be [rows, heads, head_dim]")
         rows, heads, _ = q.shape
         qs = self._rows(q, "q", rows, heads)
